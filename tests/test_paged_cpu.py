@@ -1,0 +1,148 @@
+"""The paged cache's entry points refuse bad arguments before anything is launched (no GPU
+needed: the C checks see only numbers and pointers, the wrappers only shapes and types)."""
+import ctypes as C
+
+import pytest
+import torch
+
+from vx27_b200 import ops
+
+P = C.c_void_p
+HD = 256
+
+
+def _call(vxlib, name, args):
+    err = C.create_string_buffer(256)
+    rc = getattr(vxlib, name)(*args, None, err, 256)
+    return rc, err.value.decode()
+
+
+def _append(**o):
+    a = dict(q=P(16), k=P(16), v=P(16), qw=P(16), kw=P(16), rope=P(16), rl=64, pos=P(4), slots=P(4),
+             seq=None, table=P(4), ns=2, mp=4, kp=P(16), vp=P(16), n_pages=8, ps=16, qo=P(16), n=2,
+             nq=24, nkv=4, hd=HD, rd=64, eps=1e-6, flags=0)
+    a.update(o)
+    return list(a.values())
+
+
+def _decode(**o):
+    a = dict(q=P(16), gate=None, kp=P(16), vp=P(16), n_pages=8, ps=16, table=P(4), mp=4, lens=P(4),
+             window=0, sinks=0, wsum=None, out=P(16), ws=P(16), wsb=1 << 30, B=2, nq=24, nkv=4,
+             hd=HD, splits=0, flags=0)
+    a.update(o)
+    return list(a.values())
+
+
+def _prefill(**o):
+    a = dict(q=P(16), gate=None, kp=P(16), vp=P(16), n_pages=8, ps=16, table=P(4), mp=4, s0=0,
+             window=0, sinks=0, out=P(16), ws=P(16), wsb=1 << 30, T=8, nq=24, nkv=4, hd=HD, flags=3)
+    a.update(o)
+    return list(a.values())
+
+
+def _evict(**o):
+    a = dict(kp=P(16), vp=P(32), n_pages=8, ps=16, table=P(4), mp=4, lens=P(4), ws=P(4),
+             table2=P(8), mp2=2, lens2=P(8), ws2=P(8), kept=P(4), keep=20, sinks=4, recent=8, B=2,
+             nkv=4, hd=HD)
+    a.update(o)
+    return list(a.values())
+
+
+POOL = [(dict(hd=128), "hd=128"), (dict(ps=48), "page_size=48"), (dict(ps=8), "page_size=8"),
+        (dict(ps=512), "page_size=512"), (dict(n_pages=0), "bad shape"), (dict(mp=0), "bad shape"),
+        (dict(kp=None), "null pointer"), (dict(table=None), "null pointer"),
+        (dict(kp=P(8)), "16-byte aligned"), (dict(nkv=0), "nkv=0"),
+        (dict(n_pages=1 << 26), "over 2\\^31 rows"), (dict(mp=1 << 28), "over 2\\^31 rows")]
+HEADS = [(dict(nq=36), "1 to 8 query heads"), (dict(nq=25), "1 to 8 query heads"),
+         (dict(nq=0), "1 to 8 query heads")]
+WINDOW = [(dict(window=-1), "window=-1"), (dict(window=4, sinks=-1), "sinks=-1"),
+          (dict(sinks=4), "sinks need a window")]
+
+
+@pytest.mark.parametrize("name,make,cases", [
+    ("vx27_gqa_paged_append", _append, POOL + HEADS + [
+        (dict(n=0), "n=0"), (dict(n=3), "3 tokens for 2 sequences"), (dict(rd=24), "rope_dim=24"),
+        (dict(rd=272), "rope_dim=272"), (dict(rope=None), "null pointer"),
+        (dict(q=P(8)), "16-byte aligned"), (dict(slots=None), "null pointer")]),
+    ("vx27_gqa_paged_decode", _decode, POOL + HEADS + WINDOW + [
+        (dict(B=0), "B=0"), (dict(B=65536), "B=65536"), (dict(lens=None), "null pointer"),
+        (dict(ws=None), "null pointer"), (dict(wsb=0), "workspace of 0 bytes"),
+        (dict(out=P(24)), "16-byte aligned")]),
+    ("vx27_gqa_paged_prefill", _prefill, POOL + HEADS + WINDOW + [
+        (dict(flags=1), "must be bf16"), (dict(flags=2), "must be bf16"), (dict(T=0), "slots"),
+        (dict(T=65), "slots \\[0, 0 \\+ 65\\)"), (dict(s0=-1), "slots"),
+        (dict(s0=0x7ffffff0, T=64), "slots"), (dict(wsb=100), "workspace of 100 bytes")]),
+    ("vx27_kv_evict", _evict, POOL + [
+        (dict(B=0), "B=0"), (dict(keep=0), "keep=0"), (dict(recent=17), "keep=20"),
+        (dict(sinks=-1), "keep=20"), (dict(sinks=0x7fffffff, recent=0x7fffffff), "keep=20"),
+        (dict(mp2=1), "1 pages"), (dict(mp2=0), "0 pages"), (dict(ws=None), "null pointer"),
+        (dict(table2=P(4)), "an output is an input"), (dict(lens2=P(4)), "an output is an input"),
+        (dict(ws2=P(4)), "an output is an input"), (dict(vp=P(16)), "an output is an input")]),
+])
+def test_c_refusals(vxlib, name, make, cases):
+    import re
+    for change, message in cases:
+        rc, err = _call(vxlib, name, make(**change))
+        assert rc == -1 and re.search(message, err), (name, change, rc, err)
+
+
+def test_workspace_sizes(vxlib):
+    assert ops.gqa_paged_prefill_workspace_bytes(4, HD) == 2 * 4 * 64 * 512
+    assert ops.gqa_paged_workspace_bytes(0, 24, 4, HD, 64) == 0
+    big = ops.gqa_paged_workspace_bytes(64, 24, 4, HD, 4096, weights=True)
+    assert 0 < ops.gqa_paged_workspace_bytes(1, 24, 4, HD, 64) <= big < 1 << 31
+
+
+def test_wrapper_refusals():
+    E = ops.Vx27Error
+    B, nq, nkv, ps, mp = 2, 24, 4, 16, 4
+    bf = torch.bfloat16
+    kp = torch.zeros(8, nkv, ps, HD, dtype=bf)
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    q, out, ws = torch.zeros(B, nq, HD), torch.zeros(B, nq, HD), torch.zeros(64)
+    dec = lambda **o: ops.gqa_paged_decode(**(dict(  # noqa: E731
+        q=q, gate=None, k_pages=kp, v_pages=kp, page_table=i(B, mp), lens=i(B), out=out,
+        workspace=ws) | o))
+    for change, message in [
+            (dict(k_pages=kp.float()), "k_pages: dtype"), (dict(v_pages=kp[:4]), "v_pages: shape"),
+            (dict(q=q.to(bf)), "q: dtype"), (dict(gate=q[:1]), "gate: shape"),
+            (dict(page_table=i(B + 1, mp)), "page_table: shape"),
+            (dict(page_table=i(B, mp).long()), "page_table: dtype"),
+            (dict(lens=i(B + 1)), "lens: shape"), (dict(out=out.double()), "out: dtype"),
+            (dict(weight_sum=torch.zeros(B, nkv, 8)), "weight_sum: shape"),
+            (dict(), "expected a contiguous CUDA tensor")]:
+        with pytest.raises(E, match=message):
+            dec(**change)
+    n = 3
+    x, kv = torch.zeros(n, nq, HD, dtype=bf), torch.zeros(n, nkv, HD, dtype=bf)
+    app = lambda **o: ops.gqa_paged_append(**(dict(  # noqa: E731
+        q_in=x, k_in=kv, v_in=kv, q_norm_w=torch.zeros(HD), k_norm_w=torch.zeros(HD),
+        rope=torch.zeros(8, 64), pos=i(n), slots=i(n), page_table=i(n, mp), k_pages=kp, v_pages=kp,
+        q_out=x) | o))
+    for change, message in [
+            (dict(k_in=kv.float()), "k_in: dtype"), (dict(v_in=kv[:, :2]), "v_in: shape"),
+            (dict(pos=i(n + 1)), "pos: shape"), (dict(seq=i(n).long()), "seq: dtype"),
+            (dict(q_out=x.half()), "q_out: dtype"), (dict(rope=torch.zeros(64)), "rope: shape"),
+            (dict(q_norm_w=torch.zeros(8)), "q_norm_w: 8 elements"),
+            (dict(page_table=i(mp)), "page_table: shape")]:
+        with pytest.raises(E, match=message):
+            app(**change)
+    y = torch.zeros(n, nq, HD, dtype=bf)
+    pre = lambda **o: ops.gqa_paged_prefill(**(dict(  # noqa: E731
+        q=x, gate=None, k_pages=kp, v_pages=kp, page_table=i(mp), out=y, workspace=ws) | o))
+    for change, message in [
+            (dict(q=x.float()), "q: dtype"), (dict(gate=x.float()), "gate: dtype"),
+            (dict(out=y.float()), "out: dtype"), (dict(page_table=i(1, mp)), "page_table: shape")]:
+        with pytest.raises(E, match=message):
+            pre(**change)
+    ev = lambda **o: ops.kv_evict(**(dict(  # noqa: E731
+        k_pages=kp, v_pages=kp, page_table=i(B, mp), lens=i(B),
+        weight_sum=torch.zeros(B, nkv, mp * ps), page_table_out=i(B, 2), lens_out=i(B),
+        weight_sum_out=torch.zeros(B, nkv, 2 * ps), kept=i(B, nkv, 20), keep=20) | o))
+    for change, message in [
+            (dict(weight_sum=torch.zeros(B, nkv, ps)), "weight_sum: shape"),
+            (dict(weight_sum_out=torch.zeros(B, nkv, ps)), "weight_sum_out: shape"),
+            (dict(kept=i(B, nkv, 21)), "kept: shape"), (dict(lens_out=i(1)), "lens_out: shape"),
+            (dict(page_table_out=i(1, 2)), "page_table_out: shape")]:
+        with pytest.raises(E, match=message):
+            ev(**change)

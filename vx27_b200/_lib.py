@@ -77,6 +77,17 @@ PROTOTYPES: dict[str, tuple] = {
     "vx27_gqa_partial": (_i, [_p, _p, _p, _i, _i, _i, _p, _i, _i, _i, _i, _p, _sz, _p, _cp,
                               _sz]),
     "vx27_gqa_combine": (_i, [_p, _i, _sz, _p, _p, _i, _i, _i, _i, _p, _cp, _sz]),
+    # vx27_paged.h
+    "vx27_gqa_paged_append": (_i, [_p, _p, _p, _p, _p, _p, _i, _p, _p, _p, _p, _i, _i, _p, _p, _i,
+                                   _i, _p, _i, _i, _i, _i, _i, _f, _i, _p, _cp, _sz]),
+    "vx27_gqa_paged_workspace_size": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i, _i]),
+    "vx27_gqa_paged_decode": (_i, [_p, _p, _p, _p, _i, _i, _p, _i, _p, _i, _i, _p, _p, _p, _sz,
+                                   _i, _i, _i, _i, _i, _i, _p, _cp, _sz]),
+    "vx27_gqa_paged_prefill_workspace_size": (_sz, [_i, _i]),
+    "vx27_gqa_paged_prefill": (_i, [_p, _p, _p, _p, _i, _i, _p, _i, _i, _i, _i, _p, _p, _sz, _i,
+                                    _i, _i, _i, _i, _p, _cp, _sz]),
+    "vx27_kv_evict": (_i, [_p, _p, _i, _i, _p, _i, _p, _p, _p, _i, _p, _p, _p, _i, _i, _i, _i, _i,
+                           _i, _p, _cp, _sz]),
     # vx27_pmat.h
     "vx27_pmat_row_bytes": (_sz, [C.c_uint32, _i]),
     "vx27_pmat_batch_dev": (_i, [_p, C.c_uint32, _p, _p, _i, _i, _i, _p, _cp, _sz]),

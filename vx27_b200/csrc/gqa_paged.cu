@@ -1,0 +1,420 @@
+// GQA over the paged KV cache: append and attention (include/vx27_paged.h).
+#include <math.h>
+#include <algorithm>
+#include "common.cuh"
+#include "paged.cuh"
+#include "../../include/vx27_paged.h"
+
+namespace vx27 {
+namespace {
+
+constexpr int HD = PG_HD;
+
+// 8 consecutive activations.
+template <bool BF16>
+__device__ __forceinline__ void ld8(float (&x)[8], const void *p, size_t i) {
+    if constexpr (BF16) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + i);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            x[2 * k] = bf16_to_f32(w[k] & 0xffffu);
+            x[2 * k + 1] = bf16_to_f32(w[k] >> 16);
+        }
+    } else {
+        const float4 *f = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
+        const float4 a = f[0], b = f[1];
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    }
+}
+__device__ __forceinline__ void st8_bf16(uint16_t *p, const float (&x)[8]) {
+    *reinterpret_cast<uint4 *>(p) =
+        make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
+                   pack_bf16x2(x[6], x[7]));
+}
+__device__ __forceinline__ void st8_f32(float *p, const float (&x)[8]) {
+    float4 *d = reinterpret_cast<float4 *>(p);
+    d[0] = make_float4(x[0], x[1], x[2], x[3]);
+    d[1] = make_float4(x[4], x[5], x[6], x[7]);
+}
+
+// ---- append ---------------------------------------------------------------------------
+// One warp per (token, head) row, 8 consecutive dims per lane; y = x * rsqrt(mean x^2 + eps)
+// * w, then the rotation (x0, x1) -> (x0 c - x1 s, x0 s + x1 c) of dims (i, i + rope_dim/2),
+// whose partner is rope_dim/16 lanes away. The square sum is a tree of fp32 sums.
+struct AppendArgs {
+    const void *q_in, *k_in, *v_in;
+    const float *qw, *kw, *rope;
+    const int *pos, *slots, *seq, *table;
+    uint16_t *kp, *vp;
+    void *q_out;
+    PagePool pool;
+    int rope_len, rope_dim, n_seqs, max_pages, n, nq;
+    float eps;
+    int one_p, q_bf16;
+};
+
+template <bool ACT_BF16>
+__global__ void __launch_bounds__(256)
+paged_append_k(const __grid_constant__ AppendArgs a, uint32_t *status) {
+    grid_dep_wait();
+    grid_dep_launch();
+    const int lane = threadIdx.x & 31, d0 = lane * 8;
+    const int nkv = a.pool.nkv, nh = a.nq + nkv;
+    const long long n_rows = (long long)a.n * nh;
+    const int half = a.rope_dim / 2;
+    const bool rot = d0 < a.rope_dim, lo = d0 < half;
+    const int i0 = lo ? d0 : d0 - half;
+    const int partner = (lo ? lane + half / 8 : lane - half / 8) & 31;
+    for (long long item = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; item < n_rows;
+         item += ((long long)gridDim.x * blockDim.x) >> 5) {
+        const int t = (int)(item / nh), head = (int)(item % nh);
+        const bool is_q = head < a.nq;
+        const int h = is_q ? head : head - a.nq;
+        const size_t row = (is_q ? (size_t)t * a.nq + h : (size_t)t * nkv + h) * HD + d0;
+        float x[8], v[8];
+        ld8<ACT_BF16>(x, is_q ? a.q_in : a.k_in, row);
+        const int p = a.pos[t];
+        const bool p_ok = p >= 0 && p < a.rope_len;
+        size_t dst = 0;
+        bool store = false;
+        if (!is_q) {
+            const int slot = a.slots[t], b = a.seq ? a.seq[t] : t;
+            if (slot >= 0) {
+                bool ok = b >= 0 && b < a.n_seqs && (slot >> a.pool.ps_log) < a.max_pages;
+                const int page =
+                    ok ? a.table[(size_t)b * a.max_pages + (slot >> a.pool.ps_log)] : -1;
+                ok = ok && a.pool.has(page);
+                if (!ok) dev_flag(status, VX_DEV_BAD_ARG);
+                store = ok;
+                if (ok) dst = a.pool.row(page, h, slot) * HD + d0;
+            }
+            ld8<ACT_BF16>(v, a.v_in, row);
+        }
+        float c[8], s[8];
+        if (rot && p_ok) {
+            const float *rr = a.rope + (size_t)p * a.rope_dim + i0;
+            ld8<false>(c, rr, 0);
+            ld8<false>(s, rr, half);
+        }
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) ss = fmaf(x[e], x[e], ss);
+        ss = warp_sum(ss);
+        const float r = __fdiv_rn(1.0f, __fsqrt_rn(ss * (1.0f / HD) + a.eps));
+        const float *wp = (is_q ? a.qw : a.kw) + d0;
+        float y[8], yp[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float w = __ldg(wp + e);
+            y[e] = x[e] * r * (a.one_p ? w + 1.0f : w);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) yp[e] = __shfl_sync(0xffffffffu, y[e], partner);
+        if (rot) {
+            if (!p_ok) {
+                dev_flag(status, VX_DEV_BAD_ARG);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    y[e] = lo ? fmaf(y[e], c[e], -yp[e] * s[e]) : fmaf(yp[e], s[e], y[e] * c[e]);
+            }
+        }
+        if (is_q) {
+            if (a.q_bf16) st8_bf16(static_cast<uint16_t *>(a.q_out) + row, y);
+            else st8_f32(static_cast<float *>(a.q_out) + row, y);
+        } else if (store) {
+            st8_bf16(a.kp + dst, y);
+            st8_bf16(a.vp + dst, v);
+        }
+    }
+}
+
+// ---- attention -------------------------------------------------------------------------
+// One CTA per (query row, KV head): its 8 warps take the seen slots in turn, each with a
+// running maximum and sum per query head of the group and the 256 output dims spread over
+// the lanes; the warps' parts are joined in shared memory. With weight sums the slots are
+// gone through again with the final maximum and sum.
+struct AttnArgs {
+    const void *q, *gate;
+    const uint16_t *kp, *vp;
+    const int *table, *lens;  // lens NULL: row t holds s0 + t + 1 slots of the one sequence
+    float *wsum;
+    void *out;
+    PagePool pool;
+    int max_pages, s0, window, sinks, nq, q_bf16, gate_bf16, out_bf16;
+};
+
+template <int G>
+__global__ void __launch_bounds__(256)
+paged_attn_k(const __grid_constant__ AttnArgs a, uint32_t *status) {
+    grid_dep_wait();
+    const int t = blockIdx.x, h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int cap = a.max_pages << a.pool.ps_log;
+    int n = a.lens ? a.lens[t] : a.s0 + t + 1;
+    if (n > cap || n < 0) {
+        dev_flag(status, VX_DEV_BAD_ARG);
+        n = n < 0 ? 0 : cap;
+    }
+    const SeenSlots see(n, a.window, a.sinks);
+    const int n_seen = see.sink_end + n - see.win_begin;
+    const int *table = a.table + (a.lens ? (size_t)t * a.max_pages : 0);
+    const float sc2 = 1.4426950408889634f * 0.0625f;
+    float q[G][8], acc[G][8], m[G], l[G];
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+        const size_t i = ((size_t)t * a.nq + h * G + g) * HD + lane * 8;
+        if (a.q_bf16) ld8<true>(q[g], a.q, i);
+        else ld8<false>(q[g], a.q, i);
+        m[g] = -INFINITY;
+        l[g] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) acc[g][e] = 0.f;
+    }
+    auto row_of = [&](int i, size_t &r, int &slot) {
+        slot = i < see.sink_end ? i : see.win_begin + i - see.sink_end;
+        const int page = table[slot >> a.pool.ps_log];
+        if (!a.pool.has(page)) {
+            dev_flag(status, VX_DEV_BAD_ARG);
+            return false;
+        }
+        r = a.pool.row(page, h, slot) * HD + lane * 8;
+        return true;
+    };
+    for (int i = warp; i < n_seen; i += 8) {
+        size_t r;
+        int slot;
+        if (!row_of(i, r, slot)) continue;
+        float k[8], v[8];
+        ld8<true>(k, a.kp, r);
+        ld8<true>(v, a.vp, r);
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            float s = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) s = fmaf(q[g][e], k[e], s);
+            s = warp_sum(s) * sc2;
+            const float mn = fmaxf(m[g], s);
+            const float al = exp2f(m[g] - mn), p = exp2f(s - mn);
+            m[g] = mn;
+            l[g] = fmaf(l[g], al, p);
+#pragma unroll
+            for (int e = 0; e < 8; e++) acc[g][e] = fmaf(acc[g][e], al, p * v[e]);
+        }
+    }
+    __shared__ float sm[8][G], sl[8][G], so[8][HD];
+    const int d = threadIdx.x;
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+        __syncthreads();
+        if (lane == 0) {
+            sm[warp][g] = m[g];
+            sl[warp][g] = l[g];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) so[warp][lane * 8 + e] = acc[g][e];
+        __syncthreads();
+        float M = -INFINITY, L = 0.f, O = 0.f;
+        for (int w = 0; w < 8; w++) M = fmaxf(M, sm[w][g]);
+        for (int w = 0; w < 8; w++) {
+            if (sl[w][g] == 0.f) continue;
+            const float f = exp2f(sm[w][g] - M);
+            L = fmaf(sl[w][g], f, L);
+            O = fmaf(so[w][d], f, O);
+        }
+        float o = L > 0.f ? O / L : 0.f;
+        const size_t i = ((size_t)t * a.nq + h * G + g) * HD + d;
+        if (a.gate) {
+            const float x = a.gate_bf16 ? act_ld<true>(a.gate, i) : act_ld<false>(a.gate, i);
+            o *= 1.0f / (1.0f + expf(-x));
+        }
+        if (a.out_bf16) act_st<true>(a.out, i, o);
+        else act_st<false>(a.out, i, o);
+        m[g] = M;
+        l[g] = L > 0.f ? 1.0f / L : 0.f;
+    }
+    if (!a.wsum) return;
+    float *ws = a.wsum + ((size_t)t * a.pool.nkv + h) * cap;
+    for (int i = warp; i < n_seen; i += 8) {
+        size_t r;
+        int slot;
+        if (!row_of(i, r, slot)) continue;
+        float k[8], sum = 0.f;
+        ld8<true>(k, a.kp, r);
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            float s = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) s = fmaf(q[g][e], k[e], s);
+            sum = fmaf(exp2f(warp_sum(s) * sc2 - m[g]), l[g], sum);
+        }
+        if (lane == 0) ws[slot] += sum;
+    }
+}
+
+int launch_attn(const AttnArgs &a, int rows, cudaStream_t st, char *err, size_t errlen) {
+    const dim3 grid(rows, a.pool.nkv);
+#define VX_G(G_) \
+    case G_: VX_CK(launch_pdl(paged_attn_k<G_>, grid, dim3(256), 0, st, a, dev_status())); break;
+    switch (a.nq / a.pool.nkv) {
+        VX_G(1) VX_G(2) VX_G(3) VX_G(4) VX_G(5)
+        VX_G(6) VX_G(7) VX_G(8)
+    }
+#undef VX_G
+    return 0;
+}
+
+}  // namespace
+}  // namespace vx27
+
+using namespace vx27;
+
+extern "C" {
+
+int vx27_gqa_paged_append(const void *q_in, const void *k_in, const void *v_in,
+                          const float *q_norm_w, const float *k_norm_w, const float *rope_table,
+                          int rope_table_len, const int *pos, const int *slots, const int *seq,
+                          const int *page_table, int n_seqs, int max_pages, void *k_pages,
+                          void *v_pages, int n_pages, int page_size, void *q_out, int n, int nq,
+                          int nkv, int hd, int rope_dim, float eps, int flags, void *stream,
+                          char *err, size_t errlen) {
+    const char *fn = "vx27_gqa_paged_append";
+    if (check_pool(fn, k_pages, v_pages, n_pages, page_size, page_table, max_pages, nkv, hd, err,
+                   errlen) ||
+        check_heads(fn, nq, nkv, err, errlen))
+        return -1;
+    if (n <= 0 || n_seqs <= 0) return fail(err, errlen, "%s: n=%d n_seqs=%d", fn, n, n_seqs);
+    if (!seq && n > n_seqs)
+        return fail(err, errlen, "%s: %d tokens for %d sequences without seq", fn, n, n_seqs);
+    if (rope_dim < 0 || rope_dim > hd || (rope_dim & 15))
+        return fail(err, errlen, "%s: rope_dim=%d (a multiple of 16 up to 256)", fn, rope_dim);
+    if (!q_in || !k_in || !v_in || !q_norm_w || !k_norm_w || !pos || !slots || !q_out ||
+        (rope_dim && (!rope_table || rope_table_len <= 0)))
+        return fail(err, errlen, "%s: null pointer argument", fn);
+    if (((uintptr_t)q_in | (uintptr_t)k_in | (uintptr_t)v_in | (uintptr_t)q_out |
+         (uintptr_t)rope_table) & 15)
+        return fail(err, errlen, "%s: activations, rope_table and q_out must be 16-byte aligned", fn);
+    AppendArgs a{};
+    a.q_in = q_in;
+    a.k_in = k_in;
+    a.v_in = v_in;
+    a.qw = q_norm_w;
+    a.kw = k_norm_w;
+    a.rope = rope_table;
+    a.pos = pos;
+    a.slots = slots;
+    a.seq = seq;
+    a.table = page_table;
+    a.kp = (uint16_t *)k_pages;
+    a.vp = (uint16_t *)v_pages;
+    a.q_out = q_out;
+    a.pool = PagePool{n_pages, nkv, page_size_log(page_size)};
+    a.rope_len = rope_dim ? rope_table_len : 0x7fffffff;
+    a.rope_dim = rope_dim;
+    a.n_seqs = n_seqs;
+    a.max_pages = max_pages;
+    a.n = n;
+    a.nq = nq;
+    a.eps = eps;
+    a.one_p = (flags & VX27_F_NORM_1P) != 0;
+    a.q_bf16 = (flags & VX27_F_OUT_BF16) != 0;
+    const long long rows = (long long)n * (nq + nkv);
+    const int grid = (int)std::min<long long>((rows + 7) / 8, (long long)num_sms() * 8);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (flags & VX27_F_ACT_BF16)
+        VX_CK(launch_pdl(paged_append_k<true>, dim3(grid), dim3(256), 0, st, a, dev_status()));
+    else
+        VX_CK(launch_pdl(paged_append_k<false>, dim3(grid), dim3(256), 0, st, a, dev_status()));
+    return 0;
+}
+
+size_t vx27_gqa_paged_workspace_size(int B, int nq, int nkv, int hd, int max_slots, int window,
+                                     int sinks, int weights, int n_splits) {
+    (void)window; (void)sinks; (void)weights; (void)n_splits;
+    if (B <= 0 || nq <= 0 || nkv <= 0 || hd <= 0 || max_slots <= 0) return 0;
+    return 16;
+}
+
+int vx27_gqa_paged_decode(const float *q, const void *gate, const void *k_pages,
+                          const void *v_pages, int n_pages, int page_size, const int *page_table,
+                          int max_pages, const int *lens, int window, int sinks,
+                          float *weight_sum, void *out, void *workspace, size_t workspace_bytes,
+                          int B, int nq, int nkv, int hd, int n_splits, int flags, void *stream,
+                          char *err, size_t errlen) {
+    const char *fn = "vx27_gqa_paged_decode";
+    if (check_pool(fn, k_pages, v_pages, n_pages, page_size, page_table, max_pages, nkv, hd, err,
+                   errlen) ||
+        check_heads(fn, nq, nkv, err, errlen) || check_window(fn, window, sinks, err, errlen))
+        return -1;
+    if (B <= 0 || B > 65535) return fail(err, errlen, "%s: B=%d", fn, B);
+    if (!q || !lens || !out || !workspace) return fail(err, errlen, "%s: null pointer argument", fn);
+    if (((uintptr_t)q | (uintptr_t)gate | (uintptr_t)out | (uintptr_t)workspace) & 15)
+        return fail(err, errlen, "%s: q, gate, out and the workspace must be 16-byte aligned", fn);
+    const size_t need = vx27_gqa_paged_workspace_size(B, nq, nkv, hd, max_pages * page_size, window,
+                                                      sinks, weight_sum != nullptr, n_splits);
+    if (workspace_bytes < need)
+        return fail(err, errlen, "%s: workspace of %zu bytes, need %zu", fn, workspace_bytes, need);
+    AttnArgs a{};
+    a.q = q;
+    a.gate = gate;
+    a.kp = (const uint16_t *)k_pages;
+    a.vp = (const uint16_t *)v_pages;
+    a.table = page_table;
+    a.lens = lens;
+    a.wsum = weight_sum;
+    a.out = out;
+    a.pool = PagePool{n_pages, nkv, page_size_log(page_size)};
+    a.max_pages = max_pages;
+    a.window = window;
+    a.sinks = sinks;
+    a.nq = nq;
+    a.gate_bf16 = (flags & VX27_F_ACT_BF16) != 0;
+    a.out_bf16 = (flags & VX27_F_OUT_BF16) != 0;
+    return launch_attn(a, B, (cudaStream_t)stream, err, errlen);
+}
+
+size_t vx27_gqa_paged_prefill_workspace_size(int nkv, int hd) {
+    if (nkv <= 0 || hd <= 0) return 0;
+    return (size_t)2 * nkv * 64 * hd * sizeof(uint16_t);
+}
+
+int vx27_gqa_paged_prefill(const void *q, const void *gate, const void *k_pages,
+                           const void *v_pages, int n_pages, int page_size,
+                           const int *page_table, int max_pages, int s0, int window, int sinks,
+                           void *out, void *workspace, size_t workspace_bytes, int T, int nq,
+                           int nkv, int hd, int flags, void *stream, char *err, size_t errlen) {
+    const char *fn = "vx27_gqa_paged_prefill";
+    if (check_pool(fn, k_pages, v_pages, n_pages, page_size, page_table, max_pages, nkv, hd, err,
+                   errlen) ||
+        check_heads(fn, nq, nkv, err, errlen) || check_window(fn, window, sinks, err, errlen))
+        return -1;
+    if (!(flags & VX27_F_ACT_BF16) || !(flags & VX27_F_OUT_BF16))
+        return fail(err, errlen, "%s: q, gate and out must be bf16", fn);
+    if (T <= 0 || s0 < 0 || (long long)s0 + T > (long long)max_pages * page_size)
+        return fail(err, errlen, "%s: slots [%d, %d + %d) outside %d pages of %d", fn, s0, s0, T,
+                    max_pages, page_size);
+    if (!q || !out || !workspace) return fail(err, errlen, "%s: null pointer argument", fn);
+    if (((uintptr_t)q | (uintptr_t)gate | (uintptr_t)out | (uintptr_t)workspace) & 15)
+        return fail(err, errlen, "%s: q, gate, out and the workspace must be 16-byte aligned", fn);
+    if (workspace_bytes < vx27_gqa_paged_prefill_workspace_size(nkv, hd))
+        return fail(err, errlen, "%s: workspace of %zu bytes, need %zu", fn, workspace_bytes,
+                    vx27_gqa_paged_prefill_workspace_size(nkv, hd));
+    AttnArgs a{};
+    a.q = q;
+    a.gate = gate;
+    a.kp = (const uint16_t *)k_pages;
+    a.vp = (const uint16_t *)v_pages;
+    a.table = page_table;
+    a.out = out;
+    a.pool = PagePool{n_pages, nkv, page_size_log(page_size)};
+    a.max_pages = max_pages;
+    a.s0 = s0;
+    a.window = window;
+    a.sinks = sinks;
+    a.nq = nq;
+    a.q_bf16 = a.gate_bf16 = a.out_bf16 = 1;
+    return launch_attn(a, T, (cudaStream_t)stream, err, errlen);
+}
+
+}  // extern "C"

@@ -566,6 +566,156 @@ def gqa_prefill(q_in, k_in, v_in, gate, q_norm_w, k_norm_w, rope, k_cache, v_cac
     check(rc, e)
 
 
+# ------------------------------------------------------------ paged KV cache
+def _pool(k_pages, v_pages, hd: int) -> tuple[int, int, int]:
+    """(pages, KV heads, page size) of a pool [n_pages][nkv][page_size][hd]."""
+    bf16 = _dt()[1]
+    for t, nm in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+        if t.dim() != 4 or t.shape != k_pages.shape or t.shape[3] != hd:
+            raise Vx27Error(f"{nm}: shape {tuple(t.shape)}, expected [n_pages][nkv][page_size][{hd}]"
+                            f" for both planes")
+        _need(t, nm, 0, (bf16,))
+    return k_pages.shape[:3]
+
+
+def _shape(t, name: str, shape: tuple, dtypes) -> None:
+    """Checks a tensor argument's dtype and exact shape."""
+    _need(t, name, 0, dtypes)
+    if tuple(t.shape) != shape:
+        raise Vx27Error(f"{name}: shape {tuple(t.shape)}, expected {shape}")
+
+
+def gqa_paged_append(q_in, k_in, v_in, q_norm_w, k_norm_w, rope, pos, slots, page_table, k_pages,
+                     v_pages, q_out, seq=None, eps: float = 1e-6, norm_one_plus: bool = False,
+                     stream=None) -> None:
+    """QK norm + RoPE + K/V store of n tokens into the pages of their sequences
+    (vx27_gqa_paged_append). q_in [n, nq, hd], k_in, v_in [n, nkv, hd]; pos and slots [n]
+    int32 (a slot below 0 stores nothing), seq [n] int32 or None (token i is sequence i's);
+    page_table [n_seqs, max_pages] int32; q_out [n, nq, hd], fp32 for gqa_paged_decode or bf16
+    for gqa_paged_prefill."""
+    n, nq, hd = q_in.shape
+    f32, bf16, i32, _, _ = _dt()
+    n_pages, nkv, ps = _pool(k_pages, v_pages, hd)
+    _need(q_in, "q_in", 0, (f32, bf16))
+    for t, nm in ((k_in, "k_in"), (v_in, "v_in")):
+        _shape(t, nm, (n, nkv, hd), (q_in.dtype,))
+    _need(q_norm_w, "q_norm_w", hd, (f32,))
+    _need(k_norm_w, "k_norm_w", hd, (f32,))
+    if rope.dim() != 2:
+        raise Vx27Error(f"rope: shape {tuple(rope.shape)}, expected [positions][rope_dim]")
+    _need(rope, "rope", 0, (f32,))
+    for t, nm in ((pos, "pos"), (slots, "slots")) + (((seq, "seq"),) if seq is not None else ()):
+        _shape(t, nm, (n,), (i32,))
+    if page_table.dim() != 2:
+        raise Vx27Error(f"page_table: shape {tuple(page_table.shape)}, expected [n_seqs][max_pages]")
+    _need(page_table, "page_table", 0, (i32,))
+    _shape(q_out, "q_out", (n, nq, hd), (f32, bf16))
+    flags = (F_ACT_BF16 if _is_bf16(q_in) else 0) | (F_OUT_BF16 if _is_bf16(q_out) else 0) | \
+        (F_NORM_1P if norm_one_plus else 0)
+    e = errbuf()
+    rc = load().vx27_gqa_paged_append(_t(q_in), _t(k_in), _t(v_in), _t(q_norm_w), _t(k_norm_w),
+                                      _t(rope), rope.shape[0], _t(pos), _t(slots), _t(seq),
+                                      _t(page_table), page_table.shape[0], page_table.shape[1],
+                                      _t(k_pages), _t(v_pages), n_pages, ps, _t(q_out), n, nq, nkv,
+                                      hd, rope.shape[1], eps, flags, _stream(stream), e, 512)
+    check(rc, e)
+
+
+def gqa_paged_workspace_bytes(B: int, nq: int, nkv: int, hd: int, max_slots: int, window: int = 0,
+                              sinks: int = 0, weights: bool = False, n_splits: int = 0) -> int:
+    """Workspace of a gqa_paged_decode call over tables of max_slots = max_pages * page_size
+    slots; weights: the call adds to weight_sum."""
+    return load().vx27_gqa_paged_workspace_size(B, nq, nkv, hd, max_slots, window, sinks,
+                                                int(weights), n_splits)
+
+
+def gqa_paged_decode(q, gate, k_pages, v_pages, page_table, lens, out, workspace, window: int = 0,
+                     sinks: int = 0, weight_sum=None, n_splits: int = 0, stream=None) -> None:
+    """Attention of one token per sequence over its lens[b] slots (vx27_gqa_paged_decode), all
+    of them or the last window and the first sinks. q [B, nq, hd] fp32 (from
+    gqa_paged_append), gate [B, nq, hd] or None, out [B, nq, hd]; page_table [B, max_pages],
+    lens [B] int32. weight_sum fp32 [B, nkv, max_pages * page_size] or None: the weight each
+    slot got is added to it."""
+    B, nq, hd = q.shape
+    f32, bf16, i32, _, _ = _dt()
+    n_pages, nkv, ps = _pool(k_pages, v_pages, hd)
+    _need(q, "q", 0, (f32,))
+    if gate is not None:
+        _shape(gate, "gate", (B, nq, hd), (f32, bf16))
+    if page_table.dim() != 2 or page_table.shape[0] != B:
+        raise Vx27Error(f"page_table: shape {tuple(page_table.shape)}, expected [{B}][max_pages]")
+    _need(page_table, "page_table", 0, (i32,))
+    max_pages = page_table.shape[1]
+    _shape(lens, "lens", (B,), (i32,))
+    _shape(out, "out", (B, nq, hd), (f32, bf16))
+    if weight_sum is not None:
+        _shape(weight_sum, "weight_sum", (B, nkv, max_pages * ps), (f32,))
+    flags = (F_ACT_BF16 if gate is not None and _is_bf16(gate) else 0) | \
+        (F_OUT_BF16 if _is_bf16(out) else 0)
+    e = errbuf()
+    rc = load().vx27_gqa_paged_decode(_t(q), _t(gate), _t(k_pages), _t(v_pages), n_pages, ps,
+                                      _t(page_table), max_pages, _t(lens), window, sinks,
+                                      _t(weight_sum), _t(out), _t(workspace),
+                                      workspace.numel() * workspace.element_size(), B, nq, nkv, hd,
+                                      n_splits, flags, _stream(stream), e, 512)
+    check(rc, e)
+
+
+def gqa_paged_prefill_workspace_bytes(nkv: int, hd: int) -> int:
+    return load().vx27_gqa_paged_prefill_workspace_size(nkv, hd)
+
+
+def gqa_paged_prefill(q, gate, k_pages, v_pages, page_table, out, workspace, s0: int = 0,
+                      window: int = 0, sinks: int = 0, stream=None) -> None:
+    """Causal attention of T tokens of one sequence in slots s0 .. s0 + T - 1, already
+    appended (vx27_gqa_paged_prefill); window and sinks as for gqa_paged_decode. q, gate
+    (or None), out [T, nq, hd] bf16; page_table [max_pages] int32."""
+    T, nq, hd = q.shape
+    _, bf16, i32, _, _ = _dt()
+    n_pages, nkv, ps = _pool(k_pages, v_pages, hd)
+    _need(q, "q", 0, (bf16,))
+    if gate is not None:
+        _shape(gate, "gate", (T, nq, hd), (bf16,))
+    if page_table.dim() != 1:
+        raise Vx27Error(f"page_table: shape {tuple(page_table.shape)}, expected [max_pages]")
+    _need(page_table, "page_table", 0, (i32,))
+    _shape(out, "out", (T, nq, hd), (bf16,))
+    e = errbuf()
+    rc = load().vx27_gqa_paged_prefill(_t(q), _t(gate), _t(k_pages), _t(v_pages), n_pages, ps,
+                                       _t(page_table), page_table.shape[0], s0, window, sinks,
+                                       _t(out), _t(workspace),
+                                       workspace.numel() * workspace.element_size(), T, nq, nkv, hd,
+                                       F_ACT_BF16 | F_OUT_BF16, _stream(stream), e, 512)
+    check(rc, e)
+
+
+def kv_evict(k_pages, v_pages, page_table, lens, weight_sum, page_table_out, lens_out,
+             weight_sum_out, kept, keep: int, sinks: int = 0, recent: int = 0,
+             stream=None) -> None:
+    """Cuts every sequence back to at most keep slots per KV head (vx27_kv_evict): the first
+    sinks, the last recent, and of the others those with the largest weight_sum, copied in
+    order to the pages of page_table_out [B, max_pages_out]. kept [B, nkv, keep] int32 gets
+    their old slots (-1 behind the last)."""
+    f32, _, i32, _, _ = _dt()
+    n_pages, nkv, ps = _pool(k_pages, v_pages, 256)
+    if page_table.dim() != 2 or page_table_out.dim() != 2:
+        raise Vx27Error("page_table, page_table_out: expected [B][max_pages]")
+    (B, mp), mo = page_table.shape, page_table_out.shape[1]
+    _need(page_table, "page_table", 0, (i32,))
+    _shape(page_table_out, "page_table_out", (B, mo), (i32,))
+    _shape(lens, "lens", (B,), (i32,))
+    _shape(lens_out, "lens_out", (B,), (i32,))
+    _shape(weight_sum, "weight_sum", (B, nkv, mp * ps), (f32,))
+    _shape(weight_sum_out, "weight_sum_out", (B, nkv, mo * ps), (f32,))
+    _shape(kept, "kept", (B, nkv, keep), (i32,))
+    e = errbuf()
+    rc = load().vx27_kv_evict(_t(k_pages), _t(v_pages), n_pages, ps, _t(page_table), mp, _t(lens),
+                              _t(weight_sum), _t(page_table_out), mo, _t(lens_out),
+                              _t(weight_sum_out), _t(kept), keep, sinks, recent, B, nkv, 256,
+                              _stream(stream), e, 512)
+    check(rc, e)
+
+
 def fill_normal(t, seed: int, stream_id: int, mean: float = 0.0, std: float = 1.0,
                 offset: int = 0, stream=None) -> None:
     """t[e] = element offset+e of the seeded normal stream (seed, stream_id)."""
