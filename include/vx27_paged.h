@@ -62,18 +62,18 @@ int vx27_gqa_paged_append(const void *q_in, const void *k_in, const void *v_in,
  *   weight_sum fp32 [B][nkv][max_pages * page_size] or NULL: to the entry of each slot attended
  *   to, the softmax weights that the heads of its group gave it are added (vx27_kv_evict)
  *   workspace: vx27_gqa_paged_workspace_size(...) bytes, 16-byte aligned
- * The slots are split over the SMs, n_splits ways (0: the library's choice), and the parts
+ * The slots are split over the SMs, n_parts ways (0: the library's choice), and the parts
  * joined. With fp32 out or weight_sum, q and the softmax's weights enter the tensor cores as
  * three bf16 terms (24 bits), else as two (16 bits). The result does not depend on the other
  * sequences of the batch except through the automatic split count.
  */
 size_t vx27_gqa_paged_workspace_size(int B, int nq, int nkv, int hd, int max_slots, int window,
-                                     int sinks, int weights, int n_splits);
+                                     int sinks, int weights, int n_parts);
 int vx27_gqa_paged_decode(const float *q, const void *gate, const void *k_pages,
                           const void *v_pages, int n_pages, int page_size, const int *page_table,
                           int max_pages, const int *lens, int window, int sinks,
                           float *weight_sum, void *out, void *workspace, size_t workspace_bytes,
-                          int B, int nq, int nkv, int hd, int n_splits, int flags, void *stream,
+                          int B, int nq, int nkv, int hd, int n_parts, int flags, void *stream,
                           char *err, size_t errlen);
 
 /*

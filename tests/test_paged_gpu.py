@@ -118,15 +118,15 @@ def decode_ref(pool, q, gate, lens, window, sinks, out_bf16, three):
     return ref, tol + 1e-30, sums, stol
 
 
-def run_decode(pool, q, gate, lens, out_dtype, window=0, sinks=0, weights=None, n_splits=0,
+def run_decode(pool, q, gate, lens, out_dtype, window=0, sinks=0, weights=None, n_parts=0,
                stream=None):
     B, nq = q.shape[:2]
     ws = torch.empty(ops.gqa_paged_workspace_bytes(B, nq, pool.nkv, HD, pool.max_pages * pool.ps,
-                                                   window, sinks, weights is not None, n_splits),
+                                                   window, sinks, weights is not None, n_parts),
                      dtype=torch.uint8, device="cuda")
     out = torch.full((B, nq, HD), float("nan"), device="cuda", dtype=out_dtype)
     ops.gqa_paged_decode(q, gate, pool.k, pool.v, pool.table, i32(lens), out, ws, window=window,
-                         sinks=sinks, weight_sum=weights, n_splits=n_splits, stream=stream)
+                         sinks=sinks, weight_sum=weights, n_parts=n_parts, stream=stream)
     torch.cuda.synchronize()
     assert ops.device_status() == 0
     return out
@@ -137,12 +137,12 @@ LENS = [0, 1, 15, 16, 17, 127, 128, 129, 300, 1000]
 
 @pytest.mark.parametrize("ps", [16, 32, 64, 128, 256])
 @pytest.mark.parametrize("out", [torch.float32, BF])
-@pytest.mark.parametrize("n_splits", [0, 1, 3, 7])
-def test_decode_ragged(cuda, ps, out, n_splits):
+@pytest.mark.parametrize("n_parts", [0, 1, 3, 7])
+def test_decode_ragged(cuda, ps, out, n_parts):
     g = gen(1)
     pool = Pool(g, LENS, 4, ps)
     q, gate = normal(g, len(LENS), 24, HD), normal(g, len(LENS), 24, HD).to(BF)
-    got = run_decode(pool, q, gate, LENS, out, n_splits=n_splits)
+    got = run_decode(pool, q, gate, LENS, out, n_parts=n_parts)
     ref, tol, _, _ = decode_ref(pool, q, gate, LENS, 0, 0, out == BF, out != BF)
     close(got, ref, tol)
     assert (got[0] == 0).all()
@@ -150,8 +150,8 @@ def test_decode_ragged(cuda, ps, out, n_splits):
 
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (16, 4), (100, 4), (128, 130), (129, 1),
                                           (300, 0), (5000, 4)])
-@pytest.mark.parametrize("ps,n_splits", [(16, 0), (64, 2), (256, 1)])
-def test_decode_window(cuda, window, sinks, ps, n_splits):
+@pytest.mark.parametrize("ps,n_parts", [(16, 0), (64, 2), (256, 1)])
+def test_decode_window(cuda, window, sinks, ps, n_parts):
     """Pages that no token sees are freed (-1) and what they held is NaN."""
     g = gen(2)
     pool = Pool(g, LENS, 4, ps)
@@ -166,7 +166,7 @@ def test_decode_window(cuda, window, sinks, ps, n_splits):
             if not s & set(range(p * ps, p * ps + ps)):
                 pool.table[b, p] = -1
     q = normal(g, len(LENS), 24, HD)
-    got = run_decode(pool, q, None, LENS, torch.float32, window, sinks, n_splits=n_splits)
+    got = run_decode(pool, q, None, LENS, torch.float32, window, sinks, n_parts=n_parts)
     ref, tol, _, _ = decode_ref(pool, q, None, LENS, window, sinks, False, True)
     close(got, ref, tol)
 
@@ -189,9 +189,9 @@ def test_decode_heads_and_types(cuda, nq, nkv, out, gate):
             close(weights, sums, stol)
 
 
-@pytest.mark.parametrize("n_splits", [0, 1, 5])
+@pytest.mark.parametrize("n_parts", [0, 1, 5])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (200, 3)])
-def test_decode_weight_sums(cuda, window, sinks, n_splits):
+def test_decode_weight_sums(cuda, window, sinks, n_parts):
     """The sums grow by each slot's weights, call by call, and stay as they were elsewhere."""
     g = gen(4)
     pool = Pool(g, LENS, 4, 64)
@@ -199,7 +199,7 @@ def test_decode_weight_sums(cuda, window, sinks, n_splits):
     w = normal(g, len(LENS), 4, pool.max_pages * 64).abs()
     before = w.clone()
     for step in (1, 2):
-        run_decode(pool, q, None, LENS, torch.float32, window, sinks, w, n_splits)
+        run_decode(pool, q, None, LENS, torch.float32, window, sinks, w, n_parts)
         _, _, sums, stol = decode_ref(pool, q, None, LENS, window, sinks, False, True)
         ref = before.double() + step * sums
         close(w, ref, step * stol + 2 * U * ref)

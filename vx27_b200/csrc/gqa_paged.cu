@@ -2,7 +2,7 @@
 #include <math.h>
 #include <algorithm>
 #include "common.cuh"
-#include "paged.cuh"
+#include "gqa_paged.cuh"
 #include "../../include/vx27_paged.h"
 
 namespace vx27 {
@@ -13,30 +13,8 @@ constexpr int HD = PG_HD;
 // 8 consecutive activations.
 template <bool BF16>
 __device__ __forceinline__ void ld8(float (&x)[8], const void *p, size_t i) {
-    if constexpr (BF16) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + i);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            x[2 * k] = bf16_to_f32(w[k] & 0xffffu);
-            x[2 * k + 1] = bf16_to_f32(w[k] >> 16);
-        }
-    } else {
-        const float4 *f = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
-        const float4 a = f[0], b = f[1];
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    }
-}
-__device__ __forceinline__ void st8_bf16(uint16_t *p, const float (&x)[8]) {
-    *reinterpret_cast<uint4 *>(p) =
-        make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
-                   pack_bf16x2(x[6], x[7]));
-}
-__device__ __forceinline__ void st8_f32(float *p, const float (&x)[8]) {
-    float4 *d = reinterpret_cast<float4 *>(p);
-    d[0] = make_float4(x[0], x[1], x[2], x[3]);
-    d[1] = make_float4(x[4], x[5], x[6], x[7]);
+    if constexpr (BF16) ld8_bf16(x, static_cast<const uint16_t *>(p) + i);
+    else ld8_f32(x, static_cast<const float *>(p) + i);
 }
 
 // ---- append ---------------------------------------------------------------------------
@@ -330,17 +308,20 @@ int vx27_gqa_paged_append(const void *q_in, const void *k_in, const void *v_in,
 }
 
 size_t vx27_gqa_paged_workspace_size(int B, int nq, int nkv, int hd, int max_slots, int window,
-                                     int sinks, int weights, int n_splits) {
-    (void)window; (void)sinks; (void)weights; (void)n_splits;
-    if (B <= 0 || nq <= 0 || nkv <= 0 || hd <= 0 || max_slots <= 0) return 0;
-    return 16;
+                                     int sinks, int weights, int n_parts) {
+    if (B <= 0 || nq <= 0 || nkv <= 0 || nq % nkv || hd != HD || max_slots <= 0 || window < 0 ||
+        sinks < 0)
+        return 0;
+    DecodeArgs a{};
+    return paged_decode_layout(a, nullptr, B, nq, nkv, max_slots, window, sinks, weights != 0,
+                               paged_decode_parts(n_parts));
 }
 
 int vx27_gqa_paged_decode(const float *q, const void *gate, const void *k_pages,
                           const void *v_pages, int n_pages, int page_size, const int *page_table,
                           int max_pages, const int *lens, int window, int sinks,
                           float *weight_sum, void *out, void *workspace, size_t workspace_bytes,
-                          int B, int nq, int nkv, int hd, int n_splits, int flags, void *stream,
+                          int B, int nq, int nkv, int hd, int n_parts, int flags, void *stream,
                           char *err, size_t errlen) {
     const char *fn = "vx27_gqa_paged_decode";
     if (check_pool(fn, k_pages, v_pages, n_pages, page_size, page_table, max_pages, nkv, hd, err,
@@ -351,27 +332,30 @@ int vx27_gqa_paged_decode(const float *q, const void *gate, const void *k_pages,
     if (!q || !lens || !out || !workspace) return fail(err, errlen, "%s: null pointer argument", fn);
     if (((uintptr_t)q | (uintptr_t)gate | (uintptr_t)out | (uintptr_t)workspace) & 15)
         return fail(err, errlen, "%s: q, gate, out and the workspace must be 16-byte aligned", fn);
-    const size_t need = vx27_gqa_paged_workspace_size(B, nq, nkv, hd, max_pages * page_size, window,
-                                                      sinks, weight_sum != nullptr, n_splits);
+    DecodeArgs a{};
+    int P = paged_decode_parts(n_parts);
+    const size_t need = paged_decode_layout(a, workspace, B, nq, nkv, max_pages * page_size, window,
+                                            sinks, weight_sum != nullptr, P);
     if (workspace_bytes < need)
         return fail(err, errlen, "%s: workspace of %zu bytes, need %zu", fn, workspace_bytes, need);
-    AttnArgs a{};
     a.q = q;
     a.gate = gate;
-    a.kp = (const uint16_t *)k_pages;
-    a.vp = (const uint16_t *)v_pages;
     a.table = page_table;
     a.lens = lens;
     a.wsum = weight_sum;
     a.out = out;
     a.pool = PagePool{n_pages, nkv, page_size_log(page_size)};
     a.max_pages = max_pages;
+    a.B = B;
     a.window = window;
     a.sinks = sinks;
     a.nq = nq;
     a.gate_bf16 = (flags & VX27_F_ACT_BF16) != 0;
     a.out_bf16 = (flags & VX27_F_OUT_BF16) != 0;
-    return launch_attn(a, B, (cudaStream_t)stream, err, errlen);
+    // no more runs than the tables have tiles of 128 slots
+    const long long tiles = ((long long)max_pages * page_size + 127) / 128;
+    P = (int)std::min<long long>(P, tiles * B * nkv);
+    return launch_paged_decode(a, k_pages, v_pages, P, (cudaStream_t)stream, err, errlen);
 }
 
 size_t vx27_gqa_paged_prefill_workspace_size(int nkv, int hd) {

@@ -1,0 +1,875 @@
+// Decode attention over the paged KV cache on the tensor cores (include/vx27_paged.h).
+//
+// The seen slots of the whole batch are counted in tiles of 128 aligned slots, sequence by
+// sequence and KV head by KV head, and cut into P equal runs, one per CTA (P = the SM
+// count): a run holds whole (sequence, KV head) items and at most two cut ones. Lengths are
+// on the device, so every CTA finds its run by a scan over them. A whole item is finished
+// by its CTA (gate and rounding included); a cut one leaves a record (o / l, m, l) per part,
+// which the join kernel merges. The run, not the number of sequences or their lengths,
+// decides a CTA's work: with one CTA per item or a fixed split per sequence a ragged batch
+// waits for its longest.
+//
+// Per tile:  S^T[128 x N] = K[128 x 256] Q^T       (tcgen05, tensor memory, fp32)
+//            p = 2^(s - m), one thread per slot, running maximum m per head
+//            O^T[256 x N] = V^T[256 x 128] P^T     folded into fp32 registers
+// The N columns hold each head of the group TERMS times: q (and p) split into bf16 terms,
+// x = hi + mid (+ lo), whose products with the bf16 cache are exact in fp32. Two terms carry
+// 16 bits (bf16 output), three 24 (fp32 output, weight sums).
+//
+// What bounds it: the cache bytes, 128 KB per tile through a ring of 12 chunks of 16 KB
+// (128 slots x 64 dims) per SM. A page is a box of its own: boxes of min(page_size, 128) rows
+// where all of them are seen, boxes of 16 rows at the edges.
+//
+// Warps: 0 copies (lane i: rows 16 i .. of the tile), 1 issues the MMAs, 2-5 softmax and
+// accumulation, 6 q, gate and results. Waits are bounded (2 s).
+#include <math.h>
+#include <algorithm>
+#include "common.cuh"
+#include "paged.cuh"
+#include "tc.cuh"
+#include "gqa_paged.cuh"
+
+namespace vx27 {
+namespace {
+
+constexpr int HD = PG_HD;
+constexpr int TILE = 128;
+constexpr int NSLOT = 12;          // even: a V operand is two neighbouring chunks
+constexpr int CHUNK = 16384;       // 128 slots x 64 dims, 128-byte swizzle
+constexpr int THREADS = 224;
+constexpr int JOIN_MAX = 1024;     // runs at most (records of one item)
+
+__device__ __forceinline__ uint64_t now_ns() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+    return t;
+}
+__device__ __forceinline__ bool bar_test(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; "
+        "selp.u32 %0, 1, 0, p; }"
+        : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return ok != 0;
+}
+// Bounded wait: false when the CTA has aborted or 2 s have passed (then it aborts).
+__device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, int *abort,
+                                         uint32_t *status, uint32_t code) {
+    const uint32_t addr = smem_u32(bar);
+    uint64_t t0 = 0;
+    for (uint32_t it = 0;; ++it) {
+        uint32_t ok;
+        asm volatile(
+            "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; "
+            "selp.u32 %0, 1, 0, p; }"
+            : "=r"(ok) : "r"(addr), "r"(parity) : "memory");
+        if (ok) return true;
+        if ((it & 255) == 0) {
+            if (*(volatile int *)abort) return false;
+            const uint64_t now = now_ns();
+            if (it == 0) t0 = now;
+            else if (now - t0 > 2000000000ull) {
+                *(volatile int *)abort = 1;
+                dev_flag(status, code);
+                return false;
+            }
+        }
+    }
+}
+// N consecutive fp32 columns of this thread's tensor-memory lane, one wait.
+template <int N>
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, float (&v)[N]) {
+    if constexpr (N == 32) {
+        uint32_t r[32];
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+            asm volatile(
+                "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,"
+                "%12,%13,%14,%15}, [%16];"
+                : "=r"(r[16 * k]), "=r"(r[16 * k + 1]), "=r"(r[16 * k + 2]), "=r"(r[16 * k + 3]),
+                  "=r"(r[16 * k + 4]), "=r"(r[16 * k + 5]), "=r"(r[16 * k + 6]),
+                  "=r"(r[16 * k + 7]), "=r"(r[16 * k + 8]), "=r"(r[16 * k + 9]),
+                  "=r"(r[16 * k + 10]), "=r"(r[16 * k + 11]), "=r"(r[16 * k + 12]),
+                  "=r"(r[16 * k + 13]), "=r"(r[16 * k + 14]), "=r"(r[16 * k + 15])
+                : "r"(taddr + 16 * k));
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+    } else {
+        tmem_ld16(taddr, v);
+    }
+}
+// The largest value of the warp (the sm_100a reduction over fp32; NaN loses).
+__device__ __forceinline__ float warp_max_redux(float v) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+// Byte offset of element (row, col) of a K-major operand in 128-byte swizzled rows.
+__device__ __forceinline__ uint32_t sw128(int row, int col) {
+    return (uint32_t)(row * 128 + ((((col >> 3) ^ (row & 7)) & 7) << 4) + (col & 7) * 2);
+}
+
+template <int G, int TERMS>
+struct Smem {
+    static constexpr int ROWS = (G * TERMS + 7) / 8 * 8;    // operand rows held
+    static constexpr int N = (G * TERMS + 15) / 16 * 16;    // MMA columns (rows past ROWS are
+                                                            // whatever follows, and not used)
+    static constexpr int QB = TERMS == 2 ? 2 : 1;           // q buffers
+    uint8_t ring[NSLOT][CHUNK];
+    uint8_t q[QB][4][ROWS * 128];    // 4 chunks of 64 dims
+    uint8_t p[2][2][ROWS * 128];     // 2 chunks of 64 slots
+    float ob[G][HD];                 // an item's normalised rows, for the staging warp
+    uint64_t full[NSLOT], empty[NSLOT];
+    uint64_t s_full[2], s_empty[2], p_full[2], o_full[2], o_empty[2], q_full[QB], q_empty[QB];
+    uint64_t grp[2], grp_end[2], ob_full, ob_empty, mma_done;
+    float red_max[2][4][G], red_sum[2][4][G];
+    float ml[G][2];
+    long long scan[8];               // start: sums of the warps' counts
+    long long total, run_off;        // start: all tiles; tiles of sequence run_b before the run
+    int run_b;
+    uint32_t tmem_base;
+    int abort;
+};
+static_assert(sizeof(Smem<8, 2>) + 1024 <= 232448 && sizeof(Smem<8, 3>) + 1024 <= 232448, "smem");
+
+// Tiles that sequence b's slots are seen in, per KV head; the sink tiles first.
+struct SeqTiles {
+    SeenSlots see;
+    int sink_tiles, win_tile0, tiles;
+    __device__ SeqTiles(int n, int window, int sinks) : see(n, window, sinks) {
+        win_tile0 = see.win_begin / TILE;
+        sink_tiles = min((see.sink_end + TILE - 1) / TILE, win_tile0);
+        tiles = sink_tiles + (n + TILE - 1) / TILE - win_tile0;
+    }
+    __device__ int units() const { return max(tiles, 1); }  // an empty item takes a turn too
+    __device__ int first_slot(int v) const {                // of the v-th tile
+        return (v < sink_tiles ? v : win_tile0 + v - sink_tiles) * TILE;
+    }
+};
+
+// A CTA's run: items (b, h), each with its tiles [v0, v0 + cnt).
+struct Walk {
+    const DecodeArgs &a;
+    long long u, end;   // next unit, end of the run
+    int b, h, v0, cnt;
+    SeqTiles t;
+    __device__ static SeqTiles seq(const DecodeArgs &a, int b) {
+        const int cap = a.max_pages << a.pool.ps_log;
+        return SeqTiles(b < a.B ? min(max(a.lens[b], 0), cap) : 0, a.window, a.sinks);
+    }
+    __device__ Walk(const DecodeArgs &a_, long long begin, long long end_, int b_, long long off)
+        : a(a_), u(begin), end(end_), b(b_), t(seq(a_, b_)) {
+        h = (int)(off / t.units());
+        v0 = (int)(off % t.units());
+        cnt = (int)min((long long)(t.units() - v0), end - u);
+    }
+    __device__ bool done() const { return u >= end; }
+    __device__ bool empty() const { return t.tiles == 0; }
+    __device__ bool whole() const { return v0 == 0 && cnt == t.units(); }
+    __device__ void next() {
+        u += cnt;
+        if (u >= end) return;
+        v0 = 0;
+        if (++h == a.pool.nkv) {
+            h = 0;
+            b++;
+            t = seq(a, b);
+        }
+        cnt = (int)min((long long)t.units(), end - u);
+    }
+    __device__ void next_work() {  // the next item that has tiles
+        do next();
+        while (!done() && empty());
+    }
+    __device__ void skip_empty() {
+        if (!done() && empty()) next_work();
+    }
+};
+
+template <int G, int TERMS>
+__global__ void __launch_bounds__(THREADS, 1)
+paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
+                const __grid_constant__ CUtensorMap tmk16,
+                const __grid_constant__ CUtensorMap tmv16, const __grid_constant__ DecodeArgs a,
+                uint32_t *status) {
+    extern __shared__ uint8_t smem_raw[];
+    using Sm = Smem<G, TERMS>;
+    Sm &sm = *reinterpret_cast<Sm *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    constexpr int N = Sm::N, QB = Sm::QB;
+    constexpr uint32_t TM_COLS = N == 16 ? 128 : 256, TM_O = 2 * N;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int nkv = a.pool.nkv;
+
+    if (tid == 0) {
+        for (int i = 0; i < NSLOT; i++) {
+            mbar_init(&sm.full[i], 1);
+            mbar_init(&sm.empty[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&sm.s_full[i], 1);
+            mbar_init(&sm.s_empty[i], 128);
+            mbar_init(&sm.p_full[i], 128);
+            mbar_init(&sm.o_full[i], 1);
+            mbar_init(&sm.o_empty[i], 128);
+            mbar_init(&sm.grp[i], 128);
+            mbar_init(&sm.grp_end[i], 128);
+        }
+        for (int i = 0; i < QB; i++) {
+            mbar_init(&sm.q_full[i], 32);
+            mbar_init(&sm.q_empty[i], 1);
+        }
+        mbar_init(&sm.ob_full, 128);
+        mbar_init(&sm.ob_empty, 1);
+        mbar_init(&sm.mma_done, 1);
+        sm.abort = 0;
+        fence_barrier_init();
+    }
+    if (warp == 0) {
+        tmem_alloc(&sm.tmem_base, TM_COLS);
+        tmem_relinquish();
+        if (lane == 0) {
+            tma_prefetch_desc(&tmk);
+            tma_prefetch_desc(&tmv);
+        }
+    }
+    if (warp >= 2 && warp < 6) {  // operand rows that no term fills stay zero
+        uint4 *z = reinterpret_cast<uint4 *>(&sm.q[0][0][0]);
+        for (int e = tid - 64; e < (int)(sizeof(sm.q) + sizeof(sm.p)) / 16; e += 128)
+            z[e] = make_uint4(0, 0, 0, 0);
+        fence_proxy_async();
+    }
+    grid_dep_wait();  // lengths, q, cache rows come from the kernels before
+    if (tid == 0) grid_dep_launch();
+
+    // ---- the run of this CTA: tiles [c T / P, (c + 1) T / P) of the T in all ------------
+    const int cb = (a.B + THREADS - 1) / THREADS;  // consecutive sequences per thread
+    const int b_lo = min(tid * cb, a.B), b_hi = min(b_lo + cb, a.B);
+    long long mine = 0;
+    for (int b = b_lo; b < b_hi; b++) {
+        const int n = a.lens[b];
+        if (n < 0 || n > a.max_pages << a.pool.ps_log) dev_flag(status, VX_DEV_BAD_ARG);
+        mine += (long long)Walk::seq(a, b).units() * nkv;
+    }
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += x;
+    }
+    if (lane == 31) sm.scan[warp] = incl;
+    __syncthreads();
+    long long before = incl - mine, total = 0;
+    for (int w = 0; w < THREADS / 32; w++) {
+        if (w < warp) before += sm.scan[w];
+        total += sm.scan[w];
+    }
+    const int P = (int)min((long long)gridDim.x, total), c = blockIdx.x;
+    const long long begin = c < P ? (long long)c * total / P : total;
+    const long long end = c < P ? (long long)(c + 1) * total / P : total;
+    if (begin < end && begin >= before && begin < before + mine) {
+        int b = b_lo;
+        long long at = before;
+        for (;; b++) {
+            const long long k = (long long)Walk::seq(a, b).units() * nkv;
+            if (begin < at + k) break;
+            at += k;
+        }
+        sm.run_b = b;
+        sm.run_off = begin - at;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sm.tmem_base;
+    // a run's first item may have begun in an earlier run: run c1 + 1 has it joined
+    const Walk start(a, begin, end, begin < end ? sm.run_b : a.B, begin < end ? sm.run_off : 0);
+    auto owner = [&](long long u) { return (int)(((u + 1) * P - 1) / total); };
+    if (tid == 0) {
+        int4 j = make_int4(-1, 0, 0, 0);
+        if (!start.done() && start.v0 > 0) {
+            const long long s = begin - start.v0;
+            const int c1 = owner(s), c2 = owner(s + start.t.units() - 1);
+            if (c == c1 + 1) j = make_int4(start.b * nkv + start.h, c1, c2, 0);
+        }
+        a.join[c] = j;
+    }
+
+    if (warp == 0) {
+        // ---- copies: lane i < 8 has rows [16 i, 16 i + 16) of the tile ------------------
+        const int seg = min(1 << a.pool.ps_log, TILE) / 16;  // lanes of a page's share
+        const uint32_t seg_mask = (1u << seg) - 1;
+        const int lead = lane & ~(seg - 1);
+        bool ok = true;
+        int j = 0;  // chunks issued
+        // page of this lane's rows of tile v of the walk's item, -1 when none of them is seen
+        auto page_of = [&](const Walk &w, int v) {
+            if (w.done() || lane >= 8) return -1;
+            const int s = w.t.first_slot(v) + 16 * lane;
+            const SeenSlots &see = w.t.see;
+            if (!(s < see.n && s + 16 > see.win_begin) && s >= see.sink_end) return -1;
+            const int page = a.table[(size_t)w.b * a.max_pages + (s >> a.pool.ps_log)];
+            if (!a.pool.has(page)) dev_flag(status, VX_DEV_BAD_ARG);
+            return page;
+        };
+        Walk w = start;
+        w.skip_empty();
+        int v = w.done() ? 0 : w.v0;
+        int page = page_of(w, v);
+        while (!w.done() && ok) {
+            const int s = w.t.first_slot(v) + 16 * lane, h = w.h;
+            // the next tile's pages are requested before this tile waits for ring slots
+            const int page_now = page;
+            if (++v == w.v0 + w.cnt) {
+                w.next_work();
+                v = w.done() ? 0 : w.v0;
+            }
+            page = page_of(w, v);
+            const bool need = page_now >= 0 && a.pool.has(page_now);
+            const uint32_t mask = __ballot_sync(0xffffffffu, need);
+            const bool big = ((mask >> lead) & seg_mask) == seg_mask;
+            const bool issue = need && (!big || lane == lead);
+            const int y = need ? (int)a.pool.row(page_now, h, s) : 0;
+            const uint32_t bytes = __popc(mask) * 2048;
+            for (int r = 0; r < 8; r++, j++) {
+                const int slot = j % NSLOT, round = j / NSLOT;
+                if (round > 0)
+                    ok = bar_wait(&sm.empty[slot], (round - 1) & 1, &sm.abort, status,
+                                  VX_DEV_TIMEOUT_TMA);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                if (lane == 0) mbar_arrive_expect_tx(&sm.full[slot], bytes);
+                __syncwarp();
+                if (issue) {
+                    const CUtensorMap *m = r < 4 ? (big ? &tmk : &tmk16) : (big ? &tmv : &tmv16);
+                    tma_load_2d(sm.ring[slot] + lane * 2048, m, (r & 3) * 64, y, &sm.full[slot]);
+                }
+            }
+        }
+        if (*(volatile int *)&sm.abort) {  // copies in flight land before the CTA leaves
+            for (int k = max(0, j - NSLOT); k < j; k++) {
+                const uint32_t addr = smem_u32(&sm.full[k % NSLOT]);
+                for (int it = 0; it < (1 << 20); it++) {
+                    uint32_t ok2;
+                    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                                 : "=r"(ok2) : "r"(addr), "r"((uint32_t)((k / NSLOT) & 1)) : "memory");
+                    if (ok2) break;
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ---- MMAs: S(gs) chunk by chunk as K lands, O(go) half by half as P and V are there,
+        // S at most one tile ahead: a ring slot's loads are then waited for in order
+        if (lane == 0) {
+            const uint32_t id1 = idesc_bf16(128, N, false, false);
+            const uint32_t id2 = idesc_bf16(128, N, true, false);
+            const uint32_t ring0 = smem_u32(sm.ring[0]);
+            Walk w = start;
+            w.skip_empty();
+            int left = w.done() ? 0 : w.cnt;  // S tiles to go in the item
+            bool first = true;                // the item's first S: q must be there
+            int kq = 0, gs = 0, cs = 0, go = 0, ho = 0;
+            bool s_started = false, o_started = false, ok = true;
+            uint32_t spins = 0;
+            uint64_t t_idle = 0;
+            while (ok && (left > 0 || go < gs)) {
+                bool progressed = false;
+                if (go < gs) {
+                    const int bb = go & 1;
+                    if (!o_started && bar_test(&sm.p_full[bb], (go >> 1) & 1) &&
+                        (go < 2 || bar_test(&sm.o_empty[bb], ((go >> 1) - 1) & 1)))
+                        o_started = true;
+                    if (o_started) {
+                        const int j0 = 8 * go + 4 + 2 * ho, s0 = j0 % NSLOT, s1 = s0 + 1;
+                        if (bar_test(&sm.full[s0], (j0 / NSLOT) & 1) &&
+                            bar_test(&sm.full[s1], ((j0 + 1) / NSLOT) & 1)) {
+                            tc_fence_after();
+                            const uint32_t pb = smem_u32(sm.p[bb][0]);
+#pragma unroll
+                            for (int kk = 0; kk < 8; kk++)
+                                mma_bf16(tmem + TM_O + (bb * 2 + ho) * N,
+                                         sdesc_sw128(ring0 + s0 * CHUNK + kk * 2048, CHUNK, 1024),
+                                         sdesc_sw128(pb + (kk >> 2) * (Sm::ROWS * 128) + (kk & 3) * 32,
+                                                     16, 1024),
+                                         id2, kk != 0);
+                            mma_commit(&sm.empty[s0]);
+                            mma_commit(&sm.empty[s1]);
+                            progressed = true;
+                            if (++ho == 2) {
+                                mma_commit(&sm.o_full[bb]);
+                                ho = 0;
+                                o_started = false;
+                                go++;
+                            }
+                        }
+                    }
+                }
+                if (left > 0 && gs - go <= 1) {
+                    const int bb = gs & 1;
+                    if (!s_started && (!first || bar_test(&sm.q_full[kq % QB], (kq / QB) & 1)) &&
+                        (gs < 2 || bar_test(&sm.s_empty[bb], ((gs >> 1) - 1) & 1)))
+                        s_started = true;
+                    if (s_started) {
+                        const int j = 8 * gs + cs, slot = j % NSLOT;
+                        if (bar_test(&sm.full[slot], (j / NSLOT) & 1)) {
+                            tc_fence_after();
+                            const uint32_t q0 = smem_u32(sm.q[kq % QB][0]);
+#pragma unroll
+                            for (int kk = 0; kk < 4; kk++)
+                                mma_bf16(tmem + bb * N,
+                                         sdesc_sw128(ring0 + slot * CHUNK + kk * 32, 16, 1024),
+                                         sdesc_sw128(q0 + cs * (Sm::ROWS * 128) + kk * 32, 16, 1024),
+                                         id1, (cs | kk) != 0);
+                            mma_commit(&sm.empty[slot]);
+                            progressed = true;
+                            first = false;
+                            if (++cs == 4) {
+                                mma_commit(&sm.s_full[bb]);
+                                cs = 0;
+                                s_started = false;
+                                gs++;
+                                if (--left == 0) {  // the item's S MMAs are all issued
+                                    mma_commit(&sm.q_empty[kq % QB]);
+                                    kq++;
+                                    first = true;
+                                    w.next_work();
+                                    left = w.done() ? 0 : w.cnt;
+                                }
+                            }
+                        }
+                    }
+                }
+                if (progressed) {
+                    spins = 0;
+                } else if ((++spins & 255) == 0) {  // bounded like every wait
+                    if (*(volatile int *)&sm.abort) ok = false;
+                    const uint64_t now = now_ns();
+                    if (spins == 256) t_idle = now;
+                    else if (now - t_idle > 2000000000ull) {
+                        *(volatile int *)&sm.abort = 1;
+                        dev_flag(status, VX_DEV_TIMEOUT_MMA);
+                        ok = false;
+                    }
+                }
+            }
+            mma_commit(&sm.mma_done);
+            for (int it = 0; it < (1 << 20); it++)  // also after an abort
+                if (bar_test(&sm.mma_done, 0)) break;
+        }
+    } else if (warp < 6) {
+        // ---- softmax: thread = slot r of the tile; then output dims r and r + 128 ----------
+        const int q4 = warp & 3, r = q4 * 32 + lane;
+        const uint32_t lane_addr = tmem + ((uint32_t)(q4 * 32) << 16);
+        const float sc2 = 1.4426950408889634f * 0.0625f;  // log2(e) / sqrt(256)
+        bool ok = true;
+        int g = 0, kq = 0;  // tiles and items so far
+        Walk w = start;
+        w.skip_empty();
+        for (; !w.done() && ok; w.next_work()) {
+            float m2[G], l[G], acc_a[G], acc_b[G], al[G], al_prev[G];
+#pragma unroll
+            for (int h = 0; h < G; h++) {
+                m2[h] = -INFINITY;
+                l[h] = acc_a[h] = acc_b[h] = al[h] = al_prev[h] = 0.f;
+            }
+            auto fold = [&](int t) {  // O(t), with the rescale of its tile
+                const int bb = t & 1;
+                ok = ok && bar_wait(&sm.o_full[bb], (t >> 1) & 1, &sm.abort, status,
+                                    VX_DEV_TIMEOUT_MMA);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) return;
+                tc_fence_after();
+                float oa[N], ob[N];
+                tmem_ld_cols(lane_addr + TM_O + bb * 2 * N, oa);
+                tmem_ld_cols(lane_addr + TM_O + (bb * 2 + 1) * N, ob);
+                tc_fence_before();
+                mbar_arrive(&sm.o_empty[bb]);
+#pragma unroll
+                for (int h = 0; h < G; h++) {
+                    float xa = oa[h + (TERMS - 1) * G], xb = ob[h + (TERMS - 1) * G];
+#pragma unroll
+                    for (int k = TERMS - 2; k >= 0; k--) {  // small terms first
+                        xa += oa[h + k * G];
+                        xb += ob[h + k * G];
+                    }
+                    acc_a[h] = fmaf(acc_a[h], al_prev[h], xa);
+                    acc_b[h] = fmaf(acc_b[h], al_prev[h], xb);
+                }
+            };
+            float *sc = nullptr;  // the item's scores [G][slots], for the weight sums
+            if constexpr (TERMS == 3)
+                if (a.scores)
+                    sc = a.scores + (size_t)(w.b * nkv + w.h) * G * a.score_stride;
+            for (int i = 0; i < w.cnt && ok; i++) {
+                const int gi = g + i, bb = gi & 1;
+                ok = bar_wait(&sm.s_full[bb], (gi >> 1) & 1, &sm.abort, status, VX_DEV_TIMEOUT_MMA);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
+                float s[N], x[G];
+                tmem_ld_cols(lane_addr + bb * N, s);
+                tc_fence_before();
+                mbar_arrive(&sm.s_empty[bb]);
+                const int s0 = w.t.first_slot(w.v0 + i);
+                const bool valid = w.t.see.sees(s0 + r);
+#pragma unroll
+                for (int h = 0; h < G; h++) {
+                    float t = s[h + (TERMS - 1) * G];
+#pragma unroll
+                    for (int k = TERMS - 2; k >= 0; k--) t += s[h + k * G];
+                    x[h] = valid ? t * sc2 : -INFINITY;
+                    t = warp_max_redux(x[h]);
+                    if (lane == 0) sm.red_max[bb][q4][h] = t;
+                }
+                mbar_arrive(&sm.grp[bb]);  // all four warps' maxima
+                ok = bar_wait(&sm.grp[bb], (gi >> 1) & 1, &sm.abort, status, VX_DEV_TIMEOUT_MMA);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                uint8_t *pbuf = sm.p[bb][r >> 6];
+#pragma unroll
+                for (int h = 0; h < G; h++) {
+                    const float t = fmaxf(fmaxf(sm.red_max[bb][0][h], sm.red_max[bb][1][h]),
+                                          fmaxf(sm.red_max[bb][2][h], sm.red_max[bb][3][h]));
+                    const float mn = fmaxf(m2[h], t);
+                    al[h] = exp2f(m2[h] - mn);
+                    m2[h] = mn;
+                    float p = exp2f(x[h] - mn);
+                    l[h] = fmaf(l[h], al[h], p);
+#pragma unroll
+                    for (int k = 0; k < TERMS; k++) {
+                        const uint16_t t16 = f32_to_bf16(p);
+                        *reinterpret_cast<uint16_t *>(pbuf + sw128(h + k * G, r & 63)) = t16;
+                        p -= bf16_to_f32(t16);
+                    }
+                }
+                // a tile with unseen slots: their V rows may hold anything (or not have been
+                // copied), and 0 * NaN is NaN, so they are zeroed before V^T P^T reads them. The
+                // previous O is folded first: the ring slot's load before this one has then
+                // been waited for
+                const bool part = s0 + TILE > w.t.see.n ||
+                                  (s0 < w.t.see.win_begin && s0 + TILE > w.t.see.sink_end);
+                if (part) {
+                    if (i >= 1) fold(gi - 1);
+                    for (int k = 0; k < 4 && ok; k++) {
+                        const int j = 8 * gi + 4 + k;
+                        ok = bar_wait(&sm.full[j % NSLOT], (j / NSLOT) & 1, &sm.abort, status,
+                                      VX_DEV_TIMEOUT_TMA);
+                        if (ok && !valid) {
+                            uint4 *row = reinterpret_cast<uint4 *>(sm.ring[j % NSLOT] + r * 128);
+#pragma unroll
+                            for (int e = 0; e < 8; e++) row[e] = make_uint4(0, 0, 0, 0);
+                        }
+                    }
+                }
+                fence_proxy_async();
+                mbar_arrive(&sm.p_full[bb]);
+                if (i >= 1 && !part) fold(gi - 1);
+#pragma unroll
+                for (int h = 0; h < G; h++) al_prev[h] = al[h];
+                if constexpr (TERMS == 3)
+                    if (sc && valid)
+#pragma unroll
+                        for (int h = 0; h < G; h++)
+                            sc[(size_t)h * a.score_stride + (w.v0 + i) * TILE + r] = x[h];
+            }
+            if (ok) fold(g + w.cnt - 1);
+            const int eb = kq & 1;
+#pragma unroll
+            for (int h = 0; h < G; h++) {
+                const float t = warp_sum(l[h]);
+                if (lane == 0) sm.red_sum[eb][q4][h] = t;
+            }
+            mbar_arrive(&sm.grp_end[eb]);
+            ok = bar_wait(&sm.grp_end[eb], (kq >> 1) & 1, &sm.abort, status, VX_DEV_TIMEOUT_MMA) && ok;
+            if (kq > 0)
+                ok = bar_wait(&sm.ob_empty, (kq - 1) & 1, &sm.abort, status, VX_DEV_TIMEOUT_MMA) && ok;
+            ok = __all_sync(0xffffffffu, ok);
+#pragma unroll
+            for (int h = 0; h < G; h++) {
+                const float L = sm.red_sum[eb][0][h] + sm.red_sum[eb][1][h] +
+                                sm.red_sum[eb][2][h] + sm.red_sum[eb][3][h];
+                const float inv = 1.0f / L;
+                sm.ob[h][r] = acc_a[h] * inv;
+                sm.ob[h][r + 128] = acc_b[h] * inv;
+                if (r == 0) {
+                    sm.ml[h][0] = m2[h];
+                    sm.ml[h][1] = L;
+                }
+            }
+            mbar_arrive(&sm.ob_full);
+            g += w.cnt;
+            kq++;
+        }
+    } else {
+        // ---- q in, results out --------------------------------------------------------------
+        bool ok = true;
+        int kq = 0;
+        const int d0 = 8 * lane;
+        float qv[G][8];
+        auto load_q = [&](const Walk &w) {
+#pragma unroll
+            for (int h = 0; h < G; h++)
+                ld8_f32(qv[h], a.q + ((size_t)w.b * a.nq + w.h * G + h) * HD + d0);
+        };
+        auto store_q = [&](int qb) {  // split into terms
+            uint8_t *dst = sm.q[qb][d0 >> 6];
+#pragma unroll
+            for (int h = 0; h < G; h++)
+#pragma unroll
+                for (int k = 0; k < TERMS; k++) {
+                    uint32_t wd[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        wd[e] = pack_bf16x2(qv[h][2 * e], qv[h][2 * e + 1]);
+                        qv[h][2 * e] -= bf16_to_f32(wd[e] & 0xffffu);
+                        qv[h][2 * e + 1] -= bf16_to_f32(wd[e] >> 16);
+                    }
+                    *reinterpret_cast<uint4 *>(dst + sw128(h + k * G, d0 & 63)) =
+                        make_uint4(wd[0], wd[1], wd[2], wd[3]);
+                }
+            fence_proxy_async();
+            mbar_arrive(&sm.q_full[qb]);
+        };
+        Walk nx = start;  // the item whose q is staged next
+        nx.skip_empty();
+        if (!nx.done()) {
+            load_q(nx);
+            store_q(0);
+            nx.next_work();
+        }
+        for (Walk w = start; !w.done() && ok; w.next()) {
+            const size_t base = ((size_t)w.b * a.nq + w.h * G) * HD + d0;
+            if (w.empty()) {
+#pragma unroll
+                for (int h = 0; h < G; h++) {
+                    const float z[8] = {};
+                    if (a.out_bf16) st8_bf16(static_cast<uint16_t *>(a.out) + base + h * HD, z);
+                    else st8_f32(static_cast<float *>(a.out) + base + h * HD, z);
+                }
+                continue;
+            }
+            if (!nx.done()) {
+                load_q(nx);
+                // the S MMAs of the item that used the buffer before are complete
+                if (kq + 1 >= QB)
+                    ok = bar_wait(&sm.q_empty[(kq + 1) % QB], ((kq + 1 - QB) / QB) & 1, &sm.abort,
+                                  status, VX_DEV_TIMEOUT_MMA);
+                ok = __all_sync(0xffffffffu, ok);
+                if (ok) store_q((kq + 1) % QB);
+                nx.next_work();
+            }
+            const bool whole = w.whole();
+            float gv[G][8];
+            if (whole && a.gate) {
+#pragma unroll
+                for (int h = 0; h < G; h++) {
+                    if (a.gate_bf16) ld8_bf16(gv[h], static_cast<const uint16_t *>(a.gate) + base + h * HD);
+                    else ld8_f32(gv[h], static_cast<const float *>(a.gate) + base + h * HD);
+                }
+            }
+            ok = ok && bar_wait(&sm.ob_full, kq & 1, &sm.abort, status, VX_DEV_TIMEOUT_MMA);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const size_t rec = (size_t)(2 * c + (w.v0 > 0 ? 0 : 1)) * G;
+#pragma unroll
+            for (int h = 0; h < G; h++) {
+                float o[8];
+                ld8_f32(o, &sm.ob[h][d0]);
+                if (!whole) {
+                    st8_f32(a.rec_o + (rec + h) * HD + d0, o);
+                } else {
+                    if (a.gate)
+#pragma unroll
+                        for (int e = 0; e < 8; e++) o[e] *= 1.0f / (1.0f + expf(-gv[h][e]));
+                    if (a.out_bf16) st8_bf16(static_cast<uint16_t *>(a.out) + base + h * HD, o);
+                    else st8_f32(static_cast<float *>(a.out) + base + h * HD, o);
+                }
+            }
+            const int item = w.b * nkv + w.h;
+            if (lane < G) {
+                const float2 ml = make_float2(sm.ml[lane][0], sm.ml[lane][1]);
+                if (!whole) a.rec_ml[rec + lane] = ml;
+                else if (a.scores) a.item_ml[(size_t)item * G + lane] = ml;
+            }
+            // which runs hold the item, for the weight sums
+            if (lane == 0 && a.scores && w.v0 == 0)
+                a.span[item] = make_int2(c, owner(w.u + w.t.units() - 1));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.ob_empty);
+            kq++;
+        }
+    }
+    __syncwarp();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        tmem_dealloc(tmem, TM_COLS);
+    }
+}
+
+// ---- join and weight sums ---------------------------------------------------------------
+// Blocks [0, (P - 1) G): block (c, h) merges head h of the item that run c continues, if c is
+// the second run of it: o = sum_r w_r o_r / sum_r w_r, w_r = l_r 2^(m_r - m). The other blocks
+// add the weights of 256 slots of an item: sum_h 2^(s_h - m_h) / l_h.
+__global__ void __launch_bounds__(256)
+paged_join_k(const __grid_constant__ DecodeArgs a, int P, int G, int slot_blocks) {
+    grid_dep_wait();
+    __shared__ float w_s[JOIN_MAX], red[8];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int n_join = (P - 1) * G;
+    // records of runs c1 .. c2: the first is that run's last item, the others first items
+    auto rec_of = [](int c1, int r) { return (size_t)(r == 0 ? 2 * c1 + 1 : 2 * (c1 + r)); };
+    auto block_max = [&](float m) {
+        m = warp_max(m);
+        __syncthreads();
+        if (lane == 0) red[warp] = m;
+        __syncthreads();
+        float t = red[0];
+        for (int i = 1; i < 8; i++) t = fmaxf(t, red[i]);
+        return t;
+    };
+    if ((int)blockIdx.x < n_join) {
+        const int4 j = a.join[blockIdx.x / G + 1];
+        const int h = blockIdx.x % G;
+        if (j.x < 0) return;
+        const int c1 = j.y, n = j.z - j.y + 1;
+        float m = -INFINITY;
+        for (int r = tid; r < n; r += 256) m = fmaxf(m, a.rec_ml[rec_of(c1, r) * G + h].x);
+        m = block_max(m);
+        for (int r = tid; r < n; r += 256) {
+            const float2 ml = a.rec_ml[rec_of(c1, r) * G + h];
+            w_s[r] = ml.y * exp2f(ml.x - m);
+        }
+        __syncthreads();
+        float L = 0.f, O = 0.f;
+        for (int r0 = 0; r0 < n; r0 += 8) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++)
+                v[u] = r0 + u < n ? a.rec_o[(rec_of(c1, r0 + u) * G + h) * HD + tid] : 0.f;
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const float wr = r0 + u < n ? w_s[r0 + u] : 0.f;
+                L += wr;
+                O = fmaf(wr, v[u], O);
+            }
+        }
+        float o = O / L;
+        const size_t i = ((size_t)(j.x / a.pool.nkv) * a.nq + (j.x % a.pool.nkv) * G + h) * HD + tid;
+        if (a.gate) {
+            const float g = a.gate_bf16 ? act_ld<true>(a.gate, i) : act_ld<false>(a.gate, i);
+            o *= 1.0f / (1.0f + expf(-g));
+        }
+        if (a.out_bf16) act_st<true>(a.out, i, o);
+        else act_st<false>(a.out, i, o);
+        return;
+    }
+    const int bi = blockIdx.x - n_join, item = bi / slot_blocks;
+    const int b = item / a.pool.nkv, k = (bi % slot_blocks) * 256 + tid;
+    const SeqTiles t = Walk::seq(a, b);
+    if ((bi % slot_blocks) * 256 >= t.tiles * TILE) return;
+    const int2 span = a.span[item];
+    const int n = span.y - span.x + 1;
+    const int slot = t.first_slot(k / TILE) + k % TILE;
+    const bool valid = k < t.tiles * TILE && t.see.sees(slot);
+    const float *sc = a.scores + (size_t)item * G * a.score_stride + k;
+    float sum = 0.f;
+    for (int h = 0; h < G; h++) {
+        float m, L;
+        if (n == 1) {
+            const float2 ml = a.item_ml[(size_t)item * G + h];
+            m = ml.x;
+            L = ml.y;
+        } else {
+            m = -INFINITY;
+            for (int r = tid; r < n; r += 256) m = fmaxf(m, a.rec_ml[rec_of(span.x, r) * G + h].x);
+            m = block_max(m);
+            L = 0.f;
+            for (int r = 0; r < n; r++) {
+                const float2 ml = a.rec_ml[rec_of(span.x, r) * G + h];
+                L = fmaf(ml.y, exp2f(ml.x - m), L);
+            }
+        }
+        if (valid) sum += exp2f(sc[(size_t)h * a.score_stride] - m) / L;
+    }
+    if (valid) a.wsum[(size_t)item * (a.max_pages << a.pool.ps_log) + slot] += sum;
+}
+
+}  // namespace
+
+int paged_decode_parts(int n_parts) {
+    if (n_parts <= 0) n_parts = num_sms();
+    return std::min(n_parts, JOIN_MAX);
+}
+
+// Slots that an item's scores may take: the table's, or the sinks' and the window's tiles.
+static size_t score_slots(int max_slots, int window, int sinks) {
+    const long long all = ((long long)max_slots + TILE - 1) / TILE;
+    if (!window) return (size_t)all * TILE;
+    const long long w = ((long long)window + TILE - 1) / TILE + 1 + ((long long)sinks + TILE - 1) / TILE;
+    return (size_t)std::min(all, w) * TILE;
+}
+
+size_t paged_decode_layout(DecodeArgs &a, void *workspace, int B, int nq, int nkv, int max_slots,
+                           int window, int sinks, bool weights, int P) {
+    const size_t G = nq / nkv;
+    char *p = (char *)workspace;
+    size_t off = 0;
+    auto take = [&](size_t bytes) {
+        char *at = p ? p + off : nullptr;
+        off += (bytes + 15) & ~(size_t)15;
+        return at;
+    };
+    a.join = (int4 *)take((size_t)P * sizeof(int4));
+    a.rec_o = (float *)take((size_t)2 * P * G * HD * sizeof(float));
+    a.rec_ml = (float2 *)take((size_t)2 * P * G * sizeof(float2));
+    a.scores = nullptr;
+    a.score_stride = 0;
+    if (weights) {
+        a.span = (int2 *)take((size_t)B * nkv * sizeof(int2));
+        a.item_ml = (float2 *)take((size_t)B * nq * sizeof(float2));
+        a.score_stride = score_slots(max_slots, window, sinks);
+        a.scores = (float *)take((size_t)B * nq * a.score_stride * sizeof(float));
+    }
+    return off;
+}
+
+int launch_paged_decode(const DecodeArgs &a, const void *k_pages, const void *v_pages, int P,
+                        cudaStream_t st, char *err, size_t errlen) {
+    const uint64_t rows = (uint64_t)a.pool.n_pages * a.pool.nkv << a.pool.ps_log;
+    const uint32_t box = std::min(1 << a.pool.ps_log, TILE);
+    CUtensorMap mk, mv, mk16, mv16;
+    if (make_tmap_bf16_2d(&mk, k_pages, rows, HD, HD * 2, 64, box, err, errlen) ||
+        make_tmap_bf16_2d(&mv, v_pages, rows, HD, HD * 2, 64, box, err, errlen) ||
+        make_tmap_bf16_2d(&mk16, k_pages, rows, HD, HD * 2, 64, 16, err, errlen) ||
+        make_tmap_bf16_2d(&mv16, v_pages, rows, HD, HD * 2, 64, 16, err, errlen))
+        return -1;
+    const int G = a.nq / a.pool.nkv;
+    const int slot_blocks = a.scores ? (int)((a.score_stride + 255) / 256) : 0;
+    const long long blocks = (long long)(P - 1) * G + (long long)slot_blocks * a.B * a.pool.nkv;
+    if (blocks > 0x7fffffffLL)
+        return fail(err, errlen, "vx27_gqa_paged_decode: weight sums over %d sequences of %zu slots",
+                    a.B, a.score_stride);
+    const bool three = !a.out_bf16 || a.scores;
+#define VX_D(G_, T_)                                                                          \
+    {                                                                                         \
+        const size_t smem = sizeof(Smem<G_, T_>) + 1024;                                      \
+        if (ensure_smem_attr((const void *)paged_decode_tc<G_, T_>, smem, err, errlen))       \
+            return -1;                                                                        \
+        VX_CK(launch_pdl(paged_decode_tc<G_, T_>, dim3(P), dim3(THREADS), smem, st, mk, mv, mk16, \
+                         mv16, a, dev_status()));                                             \
+    }
+#define VX_G(G_) \
+    case G_: if (three) VX_D(G_, 3) else VX_D(G_, 2) break;
+    switch (G) {
+        VX_G(1) VX_G(2) VX_G(3) VX_G(4) VX_G(5)
+        VX_G(6) VX_G(7) VX_G(8)
+    }
+#undef VX_G
+#undef VX_D
+    if (blocks > 0)
+        VX_CK(launch_pdl(paged_join_k, dim3((unsigned)blocks), dim3(256), 0, st, a, P, G, slot_blocks));
+    return 0;
+}
+
+}  // namespace vx27

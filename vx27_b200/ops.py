@@ -622,15 +622,15 @@ def gqa_paged_append(q_in, k_in, v_in, q_norm_w, k_norm_w, rope, pos, slots, pag
 
 
 def gqa_paged_workspace_bytes(B: int, nq: int, nkv: int, hd: int, max_slots: int, window: int = 0,
-                              sinks: int = 0, weights: bool = False, n_splits: int = 0) -> int:
+                              sinks: int = 0, weights: bool = False, n_parts: int = 0) -> int:
     """Workspace of a gqa_paged_decode call over tables of max_slots = max_pages * page_size
     slots; weights: the call adds to weight_sum."""
     return load().vx27_gqa_paged_workspace_size(B, nq, nkv, hd, max_slots, window, sinks,
-                                                int(weights), n_splits)
+                                                int(weights), n_parts)
 
 
 def gqa_paged_decode(q, gate, k_pages, v_pages, page_table, lens, out, workspace, window: int = 0,
-                     sinks: int = 0, weight_sum=None, n_splits: int = 0, stream=None) -> None:
+                     sinks: int = 0, weight_sum=None, n_parts: int = 0, stream=None) -> None:
     """Attention of one token per sequence over its lens[b] slots (vx27_gqa_paged_decode), all
     of them or the last window and the first sinks. q [B, nq, hd] fp32 (from
     gqa_paged_append), gate [B, nq, hd] or None, out [B, nq, hd]; page_table [B, max_pages],
@@ -657,7 +657,7 @@ def gqa_paged_decode(q, gate, k_pages, v_pages, page_table, lens, out, workspace
                                       _t(page_table), max_pages, _t(lens), window, sinks,
                                       _t(weight_sum), _t(out), _t(workspace),
                                       workspace.numel() * workspace.element_size(), B, nq, nkv, hd,
-                                      n_splits, flags, _stream(stream), e, 512)
+                                      n_parts, flags, _stream(stream), e, 512)
     check(rc, e)
 
 
