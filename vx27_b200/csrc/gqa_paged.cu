@@ -1,5 +1,5 @@
-// GQA over the paged KV cache: append and attention (include/vx27_paged.h).
-#include <math.h>
+// GQA over the paged KV cache (include/vx27_paged.h): the append kernel, and the entry points
+// of the decode (gqa_paged_tc.cu) and prompt attention (gqa_paged_prefill.cu).
 #include <algorithm>
 #include "common.cuh"
 #include "gqa_paged.cuh"
@@ -107,140 +107,6 @@ paged_append_k(const __grid_constant__ AppendArgs a, uint32_t *status) {
             st8_bf16(a.vp + dst, v);
         }
     }
-}
-
-// ---- attention -------------------------------------------------------------------------
-// One CTA per (query row, KV head): its 8 warps take the seen slots in turn, each with a
-// running maximum and sum per query head of the group and the 256 output dims spread over
-// the lanes; the warps' parts are joined in shared memory. With weight sums the slots are
-// gone through again with the final maximum and sum.
-struct AttnArgs {
-    const void *q, *gate;
-    const uint16_t *kp, *vp;
-    const int *table, *lens;  // lens NULL: row t holds s0 + t + 1 slots of the one sequence
-    float *wsum;
-    void *out;
-    PagePool pool;
-    int max_pages, s0, window, sinks, nq, q_bf16, gate_bf16, out_bf16;
-};
-
-template <int G>
-__global__ void __launch_bounds__(256)
-paged_attn_k(const __grid_constant__ AttnArgs a, uint32_t *status) {
-    grid_dep_wait();
-    const int t = blockIdx.x, h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int cap = a.max_pages << a.pool.ps_log;
-    int n = a.lens ? a.lens[t] : a.s0 + t + 1;
-    if (n > cap || n < 0) {
-        dev_flag(status, VX_DEV_BAD_ARG);
-        n = n < 0 ? 0 : cap;
-    }
-    const SeenSlots see(n, a.window, a.sinks);
-    const int n_seen = see.sink_end + n - see.win_begin;
-    const int *table = a.table + (a.lens ? (size_t)t * a.max_pages : 0);
-    const float sc2 = 1.4426950408889634f * 0.0625f;
-    float q[G][8], acc[G][8], m[G], l[G];
-#pragma unroll
-    for (int g = 0; g < G; g++) {
-        const size_t i = ((size_t)t * a.nq + h * G + g) * HD + lane * 8;
-        if (a.q_bf16) ld8<true>(q[g], a.q, i);
-        else ld8<false>(q[g], a.q, i);
-        m[g] = -INFINITY;
-        l[g] = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; e++) acc[g][e] = 0.f;
-    }
-    auto row_of = [&](int i, size_t &r, int &slot) {
-        slot = i < see.sink_end ? i : see.win_begin + i - see.sink_end;
-        const int page = table[slot >> a.pool.ps_log];
-        if (!a.pool.has(page)) {
-            dev_flag(status, VX_DEV_BAD_ARG);
-            return false;
-        }
-        r = a.pool.row(page, h, slot) * HD + lane * 8;
-        return true;
-    };
-    for (int i = warp; i < n_seen; i += 8) {
-        size_t r;
-        int slot;
-        if (!row_of(i, r, slot)) continue;
-        float k[8], v[8];
-        ld8<true>(k, a.kp, r);
-        ld8<true>(v, a.vp, r);
-#pragma unroll
-        for (int g = 0; g < G; g++) {
-            float s = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; e++) s = fmaf(q[g][e], k[e], s);
-            s = warp_sum(s) * sc2;
-            const float mn = fmaxf(m[g], s);
-            const float al = exp2f(m[g] - mn), p = exp2f(s - mn);
-            m[g] = mn;
-            l[g] = fmaf(l[g], al, p);
-#pragma unroll
-            for (int e = 0; e < 8; e++) acc[g][e] = fmaf(acc[g][e], al, p * v[e]);
-        }
-    }
-    __shared__ float sm[8][G], sl[8][G], so[8][HD];
-    const int d = threadIdx.x;
-#pragma unroll
-    for (int g = 0; g < G; g++) {
-        __syncthreads();
-        if (lane == 0) {
-            sm[warp][g] = m[g];
-            sl[warp][g] = l[g];
-        }
-#pragma unroll
-        for (int e = 0; e < 8; e++) so[warp][lane * 8 + e] = acc[g][e];
-        __syncthreads();
-        float M = -INFINITY, L = 0.f, O = 0.f;
-        for (int w = 0; w < 8; w++) M = fmaxf(M, sm[w][g]);
-        for (int w = 0; w < 8; w++) {
-            if (sl[w][g] == 0.f) continue;
-            const float f = exp2f(sm[w][g] - M);
-            L = fmaf(sl[w][g], f, L);
-            O = fmaf(so[w][d], f, O);
-        }
-        float o = L > 0.f ? O / L : 0.f;
-        const size_t i = ((size_t)t * a.nq + h * G + g) * HD + d;
-        if (a.gate) {
-            const float x = a.gate_bf16 ? act_ld<true>(a.gate, i) : act_ld<false>(a.gate, i);
-            o *= 1.0f / (1.0f + expf(-x));
-        }
-        if (a.out_bf16) act_st<true>(a.out, i, o);
-        else act_st<false>(a.out, i, o);
-        m[g] = M;
-        l[g] = L > 0.f ? 1.0f / L : 0.f;
-    }
-    if (!a.wsum) return;
-    float *ws = a.wsum + ((size_t)t * a.pool.nkv + h) * cap;
-    for (int i = warp; i < n_seen; i += 8) {
-        size_t r;
-        int slot;
-        if (!row_of(i, r, slot)) continue;
-        float k[8], sum = 0.f;
-        ld8<true>(k, a.kp, r);
-#pragma unroll
-        for (int g = 0; g < G; g++) {
-            float s = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; e++) s = fmaf(q[g][e], k[e], s);
-            sum = fmaf(exp2f(warp_sum(s) * sc2 - m[g]), l[g], sum);
-        }
-        if (lane == 0) ws[slot] += sum;
-    }
-}
-
-int launch_attn(const AttnArgs &a, int rows, cudaStream_t st, char *err, size_t errlen) {
-    const dim3 grid(rows, a.pool.nkv);
-#define VX_G(G_) \
-    case G_: VX_CK(launch_pdl(paged_attn_k<G_>, grid, dim3(256), 0, st, a, dev_status())); break;
-    switch (a.nq / a.pool.nkv) {
-        VX_G(1) VX_G(2) VX_G(3) VX_G(4) VX_G(5)
-        VX_G(6) VX_G(7) VX_G(8)
-    }
-#undef VX_G
-    return 0;
 }
 
 }  // namespace
@@ -359,8 +225,7 @@ int vx27_gqa_paged_decode(const float *q, const void *gate, const void *k_pages,
 }
 
 size_t vx27_gqa_paged_prefill_workspace_size(int nkv, int hd) {
-    if (nkv <= 0 || hd <= 0) return 0;
-    return (size_t)2 * nkv * 64 * hd * sizeof(uint16_t);
+    return nkv <= 0 || hd != HD ? 0 : paged_prompt_workspace(nkv);
 }
 
 int vx27_gqa_paged_prefill(const void *q, const void *gate, const void *k_pages,
@@ -384,21 +249,10 @@ int vx27_gqa_paged_prefill(const void *q, const void *gate, const void *k_pages,
     if (workspace_bytes < vx27_gqa_paged_prefill_workspace_size(nkv, hd))
         return fail(err, errlen, "%s: workspace of %zu bytes, need %zu", fn, workspace_bytes,
                     vx27_gqa_paged_prefill_workspace_size(nkv, hd));
-    AttnArgs a{};
-    a.q = q;
-    a.gate = gate;
-    a.kp = (const uint16_t *)k_pages;
-    a.vp = (const uint16_t *)v_pages;
-    a.table = page_table;
-    a.out = out;
-    a.pool = PagePool{n_pages, nkv, page_size_log(page_size)};
-    a.max_pages = max_pages;
-    a.s0 = s0;
-    a.window = window;
-    a.sinks = sinks;
-    a.nq = nq;
-    a.q_bf16 = a.gate_bf16 = a.out_bf16 = 1;
-    return launch_attn(a, T, (cudaStream_t)stream, err, errlen);
+    return launch_paged_prompt(q, gate, k_pages, v_pages,
+                               PagePool{n_pages, nkv, page_size_log(page_size)}, page_table,
+                               max_pages, s0, window, sinks, out, workspace, T, nq,
+                               (cudaStream_t)stream, err, errlen);
 }
 
 }  // extern "C"

@@ -1,5 +1,5 @@
-// Decode attention over the paged cache: what its entry point (gqa_paged.cu) and its kernels
-// (gqa_paged_tc.cu) share; 8-element loads and stores of the paged kernels.
+// What the entry points of the paged cache's attention (gqa_paged.cu) and its kernels
+// (gqa_paged_tc.cu, gqa_paged_prefill.cu) share; 8-element loads and stores.
 #pragma once
 #include "common.cuh"
 #include "paged.cuh"
@@ -31,6 +31,13 @@ size_t paged_decode_layout(DecodeArgs &a, void *workspace, int B, int nq, int nk
                            int window, int sinks, bool weights, int P);
 int launch_paged_decode(const DecodeArgs &a, const void *k_pages, const void *v_pages, int P,
                         cudaStream_t st, char *err, size_t errlen);
+
+// Prompt attention: T rows in slots s0 .. of the sequence with this table row.
+size_t paged_prompt_workspace(int nkv);
+int launch_paged_prompt(const void *q, const void *gate, const void *k_pages, const void *v_pages,
+                        const PagePool &pool, const int *table, int max_pages, int s0, int window,
+                        int sinks, void *out, void *workspace, int T, int nq, cudaStream_t st,
+                        char *err, size_t errlen);
 
 __device__ __forceinline__ void ld8_bf16(float (&x)[8], const uint16_t *p) {
     const uint4 v = *reinterpret_cast<const uint4 *>(p);

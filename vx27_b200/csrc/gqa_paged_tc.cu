@@ -125,6 +125,7 @@ struct Smem {
     uint64_t grp[2], grp_end[2], ob_full, ob_empty, mma_done;
     float red_max[2][4][G], red_sum[2][4][G];
     float ml[G][2];
+    int pages[2][8];                 // pages of the tile being copied and of the next one
     long long scan[8];               // start: sums of the warps' counts
     long long total, run_off;        // start: all tiles; tiles of sequence run_b before the run
     int run_b;
@@ -302,30 +303,38 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
         const int lead = lane & ~(seg - 1);
         bool ok = true;
         int j = 0;  // chunks issued
-        // page of this lane's rows of tile v of the walk's item, -1 when none of them is seen
-        auto page_of = [&](const Walk &w, int v) {
-            if (w.done() || lane >= 8) return -1;
+        constexpr int UNSEEN = -1 - 0x7fffffff;
+        // Page of this lane's rows of tile v of the walk's item: requested a tile ahead by an
+        // asynchronous copy to shared memory (a load into a register is waited for at once
+        // where it leaves its branch).
+        auto fetch = [&](const Walk &w, int v, int g) {
+            if (w.done() || lane >= 8) return;
+            int *dst = &sm.pages[g & 1][lane];
             const int s = w.t.first_slot(v) + 16 * lane;
             const SeenSlots &see = w.t.see;
-            if (!(s < see.n && s + 16 > see.win_begin) && s >= see.sink_end) return -1;
-            const int page = a.table[(size_t)w.b * a.max_pages + (s >> a.pool.ps_log)];
-            if (!a.pool.has(page)) dev_flag(status, VX_DEV_BAD_ARG);
-            return page;
+            if ((s < see.n && s + 16 > see.win_begin) || s < see.sink_end)
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;"
+                             ::"r"(smem_u32(dst)),
+                             "l"(a.table + (size_t)w.b * a.max_pages + (s >> a.pool.ps_log)) : "memory");
+            else
+                *dst = UNSEEN;
+            asm volatile("cp.async.commit_group;" ::: "memory");
         };
         Walk w = start;
         w.skip_empty();
-        int v = w.done() ? 0 : w.v0;
-        int page = page_of(w, v);
-        while (!w.done() && ok) {
+        int v = w.done() ? 0 : w.v0, g = 0;
+        fetch(w, v, 0);
+        for (; !w.done() && ok; g++) {
             const int s = w.t.first_slot(v) + 16 * lane, h = w.h;
-            // the next tile's pages are requested before this tile waits for ring slots
-            const int page_now = page;
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            const int page_now = lane < 8 ? sm.pages[g & 1][lane] : UNSEEN;
             if (++v == w.v0 + w.cnt) {
                 w.next_work();
                 v = w.done() ? 0 : w.v0;
             }
-            page = page_of(w, v);
-            const bool need = page_now >= 0 && a.pool.has(page_now);
+            fetch(w, v, g + 1);
+            const bool need = a.pool.has(page_now);
+            if (!need && page_now != UNSEEN) dev_flag(status, VX_DEV_BAD_ARG);
             const uint32_t mask = __ballot_sync(0xffffffffu, need);
             const bool big = ((mask >> lead) & seg_mask) == seg_mask;
             const bool issue = need && (!big || lane == lead);
@@ -346,6 +355,7 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
                 }
             }
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
         if (*(volatile int *)&sm.abort) {  // copies in flight land before the CTA leaves
             for (int k = max(0, j - NSLOT); k < j; k++) {
                 const uint32_t addr = smem_u32(&sm.full[k % NSLOT]);
