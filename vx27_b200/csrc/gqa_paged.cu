@@ -220,6 +220,9 @@ int vx27_gqa_paged_decode(const float *q, const void *gate, const void *k_pages,
     a.out_bf16 = (flags & VX27_F_OUT_BF16) != 0;
     // no more runs than the tables have tiles of 128 slots
     const long long tiles = ((long long)max_pages * page_size + 127) / 128;
+    if (tiles * B * nkv > 0x7fffffffLL)
+        return fail(err, errlen, "%s: %d sequences of %d pages: over 2^31 tiles of 128 slots", fn, B,
+                    max_pages);
     P = (int)std::min<long long>(P, tiles * B * nkv);
     return launch_paged_decode(a, k_pages, v_pages, P, (cudaStream_t)stream, err, errlen);
 }

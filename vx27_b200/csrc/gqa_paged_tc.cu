@@ -16,9 +16,12 @@
 // x = hi + mid (+ lo), whose products with the bf16 cache are exact in fp32. Two terms carry
 // 16 bits (bf16 output), three 24 (fp32 output, weight sums).
 //
-// What bounds it: the cache bytes, 128 KB per tile through a ring of 12 chunks of 16 KB
-// (128 slots x 64 dims) per SM. A page is a box of its own: boxes of min(page_size, 128) rows
-// where all of them are seen, boxes of 16 rows at the edges.
+// What bounds it: the cache bytes, 128 KB per tile through a ring of 12 chunks of 16 KB (128
+// slots x 64 dims) per SM, each tile's K and then its V by one warp. (Rings of their own for K
+// and V, by two warps, read memory in a worse order: 0.75 of its bandwidth instead of 0.84 over
+// 128 sequences of 2048 slots, whatever the split of the 12 slots.) A page is a box of its own: boxes of min(page_size, 128) rows
+// where all of them are seen, else boxes of the 16-row groups with a seen slot. The O MMAs
+// take 16 slots each and leave the other groups out; unseen rows of a copied group are zeroed.
 //
 // Warps: 0 copies (lane i: rows 16 i .. of the tile), 1 issues the MMAs, 2-5 softmax and
 // accumulation, 6 q, gate and results. Waits are bounded (2 s).
@@ -34,10 +37,12 @@ namespace {
 
 constexpr int HD = PG_HD;
 constexpr int TILE = 128;
-constexpr int NSLOT = 12;          // even: a V operand is two neighbouring chunks
+constexpr int NK = 6, NV = 6;      // ring slots; NV even: a V operand is two neighbouring chunks
 constexpr int CHUNK = 16384;       // 128 slots x 64 dims, 128-byte swizzle
-constexpr int THREADS = 224;
+constexpr int THREADS = 288;
+constexpr int SM_WARP0 = 2, STAGE_WARP = 6, V_WARP = 7, O_WARP = 8;  // 0: K copies, 1: S MMAs
 constexpr int JOIN_MAX = 1024;     // runs at most (records of one item)
+constexpr int RUN_LENS = 128;      // lengths kept in shared memory
 
 __device__ __forceinline__ uint64_t now_ns() {
     uint64_t t;
@@ -52,29 +57,40 @@ __device__ __forceinline__ bool bar_test(uint64_t *bar, uint32_t parity) {
         : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
     return ok != 0;
 }
-// Bounded wait: false when the CTA has aborted or 2 s have passed (then it aborts).
+__device__ __forceinline__ bool bar_try(uint32_t addr, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; "
+        "selp.u32 %0, 1, 0, p; }"
+        : "=r"(ok) : "r"(addr), "r"(parity) : "memory");
+    return ok != 0;
+}
+// Bounded wait: false when the CTA has aborted or 2 s have passed (then it aborts). Only the
+// first try is inlined: the roles' loops share the instruction cache, and with the whole wait
+// in each of them (and 64-bit divisions in their walks) a third of the warps' time went by
+// waiting for instructions.
+__device__ __noinline__ bool bar_wait_long(uint32_t addr, uint32_t parity, int *abort,
+                                           uint32_t *status, uint32_t code) {
+    const uint64_t t0 = now_ns();
+    for (;;) {
+        if (bar_try(addr, parity)) return true;
+        if (*(volatile int *)abort) return false;
+        if (now_ns() - t0 > 2000000000ull) break;
+    }
+    *(volatile int *)abort = 1;
+    dev_flag(status, code);
+    return false;
+}
 __device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, int *abort,
                                          uint32_t *status, uint32_t code) {
     const uint32_t addr = smem_u32(bar);
-    uint64_t t0 = 0;
-    for (uint32_t it = 0;; ++it) {
-        uint32_t ok;
-        asm volatile(
-            "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; "
-            "selp.u32 %0, 1, 0, p; }"
-            : "=r"(ok) : "r"(addr), "r"(parity) : "memory");
-        if (ok) return true;
-        if ((it & 255) == 0) {
-            if (*(volatile int *)abort) return false;
-            const uint64_t now = now_ns();
-            if (it == 0) t0 = now;
-            else if (now - t0 > 2000000000ull) {
-                *(volatile int *)abort = 1;
-                dev_flag(status, code);
-                return false;
-            }
-        }
-    }
+    return bar_try(addr, parity) || bar_wait_long(addr, parity, abort, status, code);
+}
+__device__ __noinline__ int mul_div(int a, int b, int c) { return (int)((long long)a * b / c); }
+// Bounded wait that goes on after an abort: what must be done before the CTA may leave.
+__device__ __forceinline__ void bar_drain(uint64_t *bar, uint32_t parity) {
+    for (int it = 0; it < (1 << 20); it++)
+        if (bar_test(bar, parity)) return;
 }
 // N consecutive fp32 columns of this thread's tensor-memory lane, one wait.
 template <int N>
@@ -116,19 +132,20 @@ struct Smem {
     static constexpr int N = (G * TERMS + 15) / 16 * 16;    // MMA columns (rows past ROWS are
                                                             // whatever follows, and not used)
     static constexpr int QB = TERMS == 2 ? 2 : 1;           // q buffers
-    uint8_t ring[NSLOT][CHUNK];
+    uint8_t ring[NK + NV][CHUNK];    // K slots, then V slots
     uint8_t q[QB][4][ROWS * 128];    // 4 chunks of 64 dims
     uint8_t p[2][2][ROWS * 128];     // 2 chunks of 64 slots
     float ob[G][HD];                 // an item's normalised rows, for the staging warp
-    uint64_t full[NSLOT], empty[NSLOT];
-    uint64_t s_full[2], s_empty[2], p_full[2], o_full[2], o_empty[2], q_full[QB], q_empty[QB];
-    uint64_t grp[2], grp_end[2], ob_full, ob_empty, mma_done;
+    uint64_t full[NK + NV], empty[NK + NV];
+    uint64_t s_full[2], s_empty[2], p_full[2], o_full[2], o_empty[2], v_ok[2], q_full[QB], q_empty[QB];
+    uint64_t grp[2], grp_end[2], ob_full, ob_empty, mma_done[2];
     float red_max[2][4][G], red_sum[2][4][G];
     float ml[G][2];
-    int pages[2][8];                 // pages of the tile being copied and of the next one
-    long long scan[8];               // start: sums of the warps' counts
-    long long total, run_off;        // start: all tiles; tiles of sequence run_b before the run
-    int run_b;
+    int pages[2][2][8];              // K and V: of the tile being copied and of the next one
+    int scan[THREADS / 32];          // start: the warps' tiles
+    int run_b, run_off;              // start: the run's first sequence, its tiles before the run
+    int lens[RUN_LENS];              // of the run's first sequences
+    float m_fin[2][G];
     uint32_t tmem_base;
     int abort;
 };
@@ -143,48 +160,62 @@ struct SeqTiles {
         sink_tiles = min((see.sink_end + TILE - 1) / TILE, win_tile0);
         tiles = sink_tiles + (n + TILE - 1) / TILE - win_tile0;
     }
-    __device__ int units() const { return max(tiles, 1); }  // an empty item takes a turn too
     __device__ int first_slot(int v) const {                // of the v-th tile
         return (v < sink_tiles ? v : win_tile0 + v - sink_tiles) * TILE;
     }
+    // 16-slot groups of the tile at s0 that hold a slot of [from, to)
+    __device__ static uint32_t groups(int s0, int from, int to) {
+        from = max(from - s0, 0);
+        to = min(to - s0, TILE);
+        return from < to ? (2u << ((to - 1) >> 4)) - (1u << (from >> 4)) : 0u;
+    }
+    __device__ uint32_t seen_groups(int s0) const {
+        return groups(s0, see.win_begin, see.n) | groups(s0, 0, see.sink_end);
+    }
 };
 
-// A CTA's run: items (b, h), each with its tiles [v0, v0 + cnt).
+// Length of sequence b, clipped to its table.
+__device__ __forceinline__ int seq_len(const DecodeArgs &a, int b) {
+    return min(max(a.lens[b], 0), a.max_pages << a.pool.ps_log);
+}
+
+// A CTA's run: items (b, h), each with its tiles [v0, v0 + cnt). Sequences without slots are
+// not met. The lengths of the first ones are in shared memory (with the memory busy a load
+// takes as long as one or two tiles).
 struct Walk {
     const DecodeArgs &a;
-    long long u, end;   // next unit, end of the run
+    const int *lens;
+    int run_b, left;  // first sequence; tiles to go, the item's included
     int b, h, v0, cnt;
     SeqTiles t;
-    __device__ static SeqTiles seq(const DecodeArgs &a, int b) {
-        const int cap = a.max_pages << a.pool.ps_log;
-        return SeqTiles(b < a.B ? min(max(a.lens[b], 0), cap) : 0, a.window, a.sinks);
+    __device__ __forceinline__ SeqTiles seq() const {
+        const int i = b - run_b;
+        return SeqTiles(i < RUN_LENS ? lens[i] : seq_len(a, b), a.window, a.sinks);
     }
-    __device__ Walk(const DecodeArgs &a_, long long begin, long long end_, int b_, long long off)
-        : a(a_), u(begin), end(end_), b(b_), t(seq(a_, b_)) {
-        h = (int)(off / t.units());
-        v0 = (int)(off % t.units());
-        cnt = (int)min((long long)(t.units() - v0), end - u);
+    __device__ __forceinline__ Walk(const DecodeArgs &a_, const int *lens_, int run_b_, int off,
+                                    int left_)
+        : a(a_), lens(lens_), run_b(run_b_), left(left_), b(run_b_), h(0), v0(off), cnt(0),
+          t(left_ > 0 ? seq() : SeqTiles(0, 0, 0)) {
+        if (left > 0) {
+            h = off / t.tiles;
+            v0 = off % t.tiles;
+            cnt = min(t.tiles - v0, left);
+        }
     }
-    __device__ bool done() const { return u >= end; }
-    __device__ bool empty() const { return t.tiles == 0; }
-    __device__ bool whole() const { return v0 == 0 && cnt == t.units(); }
-    __device__ void next() {
-        u += cnt;
-        if (u >= end) return;
+    __device__ __forceinline__ bool done() const { return left <= 0; }
+    __device__ __forceinline__ bool whole() const { return cnt == t.tiles; }
+    __device__ __forceinline__ void next() {
+        left -= cnt;
         v0 = 0;
+        if (left <= 0) return;
         if (++h == a.pool.nkv) {
             h = 0;
-            b++;
-            t = seq(a, b);
+            do {
+                b++;
+                t = seq();
+            } while (t.tiles == 0);
         }
-        cnt = (int)min((long long)t.units(), end - u);
-    }
-    __device__ void next_work() {  // the next item that has tiles
-        do next();
-        while (!done() && empty());
-    }
-    __device__ void skip_empty() {
-        if (!done() && empty()) next_work();
+        cnt = min(t.tiles, left);
     }
 };
 
@@ -203,7 +234,7 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
     const int nkv = a.pool.nkv;
 
     if (tid == 0) {
-        for (int i = 0; i < NSLOT; i++) {
+        for (int i = 0; i < NK + NV; i++) {
             mbar_init(&sm.full[i], 1);
             mbar_init(&sm.empty[i], 1);
         }
@@ -211,6 +242,7 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
             mbar_init(&sm.s_full[i], 1);
             mbar_init(&sm.s_empty[i], 128);
             mbar_init(&sm.p_full[i], 128);
+            mbar_init(&sm.v_ok[i], 1);
             mbar_init(&sm.o_full[i], 1);
             mbar_init(&sm.o_empty[i], 128);
             mbar_init(&sm.grp[i], 128);
@@ -222,7 +254,8 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
         }
         mbar_init(&sm.ob_full, 128);
         mbar_init(&sm.ob_empty, 1);
-        mbar_init(&sm.mma_done, 1);
+        mbar_init(&sm.mma_done[0], 1);
+        mbar_init(&sm.mma_done[1], 1);
         sm.abort = 0;
         fence_barrier_init();
     }
@@ -234,7 +267,7 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
             tma_prefetch_desc(&tmv);
         }
     }
-    if (warp >= 2 && warp < 6) {  // operand rows that no term fills stay zero
+    if (warp >= SM_WARP0 && warp < STAGE_WARP) {  // operand rows that no term fills stay zero
         uint4 *z = reinterpret_cast<uint4 *>(&sm.q[0][0][0]);
         for (int e = tid - 64; e < (int)(sizeof(sm.q) + sizeof(sm.p)) / 16; e += 128)
             z[e] = make_uint4(0, 0, 0, 0);
@@ -246,33 +279,31 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
     // ---- the run of this CTA: tiles [c T / P, (c + 1) T / P) of the T in all ------------
     const int cb = (a.B + THREADS - 1) / THREADS;  // consecutive sequences per thread
     const int b_lo = min(tid * cb, a.B), b_hi = min(b_lo + cb, a.B);
-    long long mine = 0;
+    int mine = 0;
     for (int b = b_lo; b < b_hi; b++) {
         const int n = a.lens[b];
         if (n < 0 || n > a.max_pages << a.pool.ps_log) dev_flag(status, VX_DEV_BAD_ARG);
-        mine += (long long)Walk::seq(a, b).units() * nkv;
+        mine += SeqTiles(seq_len(a, b), a.window, a.sinks).tiles * nkv;
     }
-    long long incl = mine;
+    int incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, incl, o);
+        const int x = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += x;
     }
     if (lane == 31) sm.scan[warp] = incl;
     __syncthreads();
-    long long before = incl - mine, total = 0;
+    int before = incl - mine, total = 0;
     for (int w = 0; w < THREADS / 32; w++) {
         if (w < warp) before += sm.scan[w];
         total += sm.scan[w];
     }
-    const int P = (int)min((long long)gridDim.x, total), c = blockIdx.x;
-    const long long begin = c < P ? (long long)c * total / P : total;
-    const long long end = c < P ? (long long)(c + 1) * total / P : total;
+    const int P = min((int)gridDim.x, total), c = blockIdx.x;
+    const int begin = c < P ? mul_div(c, total, P) : 0, end = c < P ? mul_div(c + 1, total, P) : 0;
     if (begin < end && begin >= before && begin < before + mine) {
-        int b = b_lo;
-        long long at = before;
+        int b = b_lo, at = before;
         for (;; b++) {
-            const long long k = (long long)Walk::seq(a, b).units() * nkv;
+            const int k = SeqTiles(seq_len(a, b), a.window, a.sinks).tiles * nkv;
             if (begin < at + k) break;
             at += k;
         }
@@ -283,236 +314,318 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sm.tmem_base;
-    // a run's first item may have begun in an earlier run: run c1 + 1 has it joined
-    const Walk start(a, begin, end, begin < end ? sm.run_b : a.B, begin < end ? sm.run_off : 0);
-    auto owner = [&](long long u) { return (int)(((u + 1) * P - 1) / total); };
+    const int run_b = begin < end ? sm.run_b : 0;
+    if (tid < RUN_LENS && run_b + tid < a.B) sm.lens[tid] = seq_len(a, run_b + tid);
+    __syncthreads();
+    const Walk start(a, sm.lens, run_b, begin < end ? sm.run_off : 0, end - begin);
+    // the run that holds tile u
+    auto owner = [&](int u) { return (int)((((long long)u + 1) * P - 1) / total); };
+    // an item that began in an earlier run is joined by the block of its second run
     if (tid == 0) {
         int4 j = make_int4(-1, 0, 0, 0);
         if (!start.done() && start.v0 > 0) {
-            const long long s = begin - start.v0;
-            const int c1 = owner(s), c2 = owner(s + start.t.units() - 1);
+            const int s = begin - start.v0;
+            const int c1 = owner(s), c2 = owner(s + start.t.tiles - 1);
             if (c == c1 + 1) j = make_int4(start.b * nkv + start.h, c1, c2, 0);
         }
         a.join[c] = j;
     }
 
-    if (warp == 0) {
-        // ---- copies: lane i < 8 has rows [16 i, 16 i + 16) of the tile ------------------
+    if (warp == 0 || warp == V_WARP) {
+        // ---- copies of K (warp 0) and of V: lane i < 8 has rows [16 i, 16 i + 16) of a tile ----
+        const bool is_k = warp == 0;
+        const int ring0 = is_k ? 0 : NK, slots = is_k ? NK : NV;
         const int seg = min(1 << a.pool.ps_log, TILE) / 16;  // lanes of a page's share
         const uint32_t seg_mask = (1u << seg) - 1;
         const int lead = lane & ~(seg - 1);
-        bool ok = true;
-        int j = 0;  // chunks issued
-        constexpr int UNSEEN = -1 - 0x7fffffff;
-        // Page of this lane's rows of tile v of the walk's item: requested a tile ahead by an
-        // asynchronous copy to shared memory (a load into a register is waited for at once
-        // where it leaves its branch).
+        // The page of this lane's rows of tile v of the walk's item goes to shared memory by an
+        // asynchronous copy, a tile ahead (a load into a register is waited for at once where
+        // it leaves its branch).
         auto fetch = [&](const Walk &w, int v, int g) {
             if (w.done() || lane >= 8) return;
-            int *dst = &sm.pages[g & 1][lane];
-            const int s = w.t.first_slot(v) + 16 * lane;
-            const SeenSlots &see = w.t.see;
-            if ((s < see.n && s + 16 > see.win_begin) || s < see.sink_end)
+            const int s0 = w.t.first_slot(v);
+            if ((w.t.seen_groups(s0) >> lane) & 1)
                 asm volatile("cp.async.ca.shared.global [%0], [%1], 4;"
-                             ::"r"(smem_u32(dst)),
-                             "l"(a.table + (size_t)w.b * a.max_pages + (s >> a.pool.ps_log)) : "memory");
-            else
-                *dst = UNSEEN;
+                             ::"r"(smem_u32(&sm.pages[!is_k][g & 1][lane])),
+                             "l"(a.table + (size_t)w.b * a.max_pages +
+                                 ((s0 + 16 * lane) >> a.pool.ps_log)) : "memory");
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
+        // V rows of copied groups that are not seen may hold anything, and 0 * NaN is NaN: once
+        // the tile has landed they are zeroed. Until then the tile is due (its slots, 1 due).
+        bool due = false, ok = true;
+        int due_g = 0, due_s0 = 0;
+        SeenSlots due_see(0, 0, 0);
+        auto landed = [&]() {
+            const int j = 4 * due_g + (lane & 3);
+            return (bool)__all_sync(0xffffffffu, bar_test(&sm.full[NK + j % NV], (j / NV) & 1));
+        };
+        // V(g) may be multiplied once it has landed. It is copied over V(g - 1)'s first half, so
+        // v_ok(g - 2), on the same barrier, is over.
+        auto v_done = [&](int g) {
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.v_ok[g & 1]);
+        };
+        auto zero_edges = [&]() {
+            auto edge = [&](int at) {  // the group that slot `at` is in, unless it begins there
+                if ((at & 15) == 0 || at < due_s0 || at >= due_s0 + TILE) return;
+                for (int i = lane >> 3; i < 16; i += 4) {
+                    const int slot = (at & ~15) + i;
+                    if (due_see.sees(slot)) continue;
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        *reinterpret_cast<uint4 *>(sm.ring[NK + (4 * due_g + k) % NV] +
+                                                   (slot - due_s0) * 128 + (lane & 7) * 16) =
+                            make_uint4(0, 0, 0, 0);
+                }
+            };
+            edge(due_see.n);
+            edge(due_see.win_begin);
+            edge(due_see.sink_end);
+            due = false;
+            v_done(due_g);
+        };
+        // Waits for a ring slot (bar), or for the due tile (NULL); a due tile may land meanwhile.
+        auto wait_for = [&](uint64_t *bar, uint32_t parity) {
+            if (!due)
+                return !bar || (bool)__all_sync(0xffffffffu, bar_wait(bar, parity, &sm.abort, status,
+                                                                      VX_DEV_TIMEOUT_TMA));
+            const uint64_t t0 = now_ns();
+            for (;;) {
+                if (due && landed()) zero_edges();
+                if (bar ? (bool)__all_sync(0xffffffffu, bar_test(bar, parity)) : !due) return true;
+                bool stop = *(volatile int *)&sm.abort;
+                if (now_ns() - t0 > 2000000000ull) {
+                    *(volatile int *)&sm.abort = 1;
+                    dev_flag(status, VX_DEV_TIMEOUT_TMA);
+                    stop = true;
+                }
+                if (__any_sync(0xffffffffu, stop)) return false;
+            }
+        };
         Walk w = start;
-        w.skip_empty();
-        int v = w.done() ? 0 : w.v0, g = 0;
+        int v = w.done() ? 0 : w.v0, g = 0, j = 0;  // tiles and chunks of this ring so far
         fetch(w, v, 0);
         for (; !w.done() && ok; g++) {
-            const int s = w.t.first_slot(v) + 16 * lane, h = w.h;
+            const int s0 = w.t.first_slot(v), h = w.h;
+            const SeenSlots see = w.t.see;
+            const uint32_t seen = w.t.seen_groups(s0);
             asm volatile("cp.async.wait_all;" ::: "memory");
-            const int page_now = lane < 8 ? sm.pages[g & 1][lane] : UNSEEN;
-            if (++v == w.v0 + w.cnt) {
-                w.next_work();
-                v = w.done() ? 0 : w.v0;
-            }
-            fetch(w, v, g + 1);
-            const bool need = a.pool.has(page_now);
-            if (!need && page_now != UNSEEN) dev_flag(status, VX_DEV_BAD_ARG);
+            const int page = lane < 8 ? sm.pages[!is_k][g & 1][lane] : 0;
+            const bool want = (seen >> lane) & 1, need = want && a.pool.has(page);
+            if (want && !need) dev_flag(status, VX_DEV_BAD_ARG);
             const uint32_t mask = __ballot_sync(0xffffffffu, need);
             const bool big = ((mask >> lead) & seg_mask) == seg_mask;
             const bool issue = need && (!big || lane == lead);
-            const int y = need ? (int)a.pool.row(page_now, h, s) : 0;
+            const int y = need ? (int)a.pool.row(page, h, s0 + 16 * lane) : 0;
             const uint32_t bytes = __popc(mask) * 2048;
-            for (int r = 0; r < 8; r++, j++) {
-                const int slot = j % NSLOT, round = j / NSLOT;
-                if (round > 0)
-                    ok = bar_wait(&sm.empty[slot], (round - 1) & 1, &sm.abort, status,
-                                  VX_DEV_TIMEOUT_TMA);
-                ok = __all_sync(0xffffffffu, ok);
+            if (++v == w.v0 + w.cnt) {
+                w.next();
+                v = w.done() ? 0 : w.v0;
+            }
+            fetch(w, v, g + 1);
+            const CUtensorMap *map = is_k ? (big ? &tmk : &tmk16) : (big ? &tmv : &tmv16);
+            for (int r = 0; r < 4; r++, j++) {
+                const int slot = ring0 + j % slots, round = j / slots;
+                if (round > 0) ok = wait_for(&sm.empty[slot], (round - 1) & 1);
                 if (!ok) break;
                 if (lane == 0) mbar_arrive_expect_tx(&sm.full[slot], bytes);
                 __syncwarp();
-                if (issue) {
-                    const CUtensorMap *m = r < 4 ? (big ? &tmk : &tmk16) : (big ? &tmv : &tmv16);
-                    tma_load_2d(sm.ring[slot] + lane * 2048, m, (r & 3) * 64, y, &sm.full[slot]);
-                }
+                if (issue) tma_load_2d(sm.ring[slot] + lane * 2048, map, r * 64, y, &sm.full[slot]);
+            }
+            if (is_k || !ok) continue;
+            ok = wait_for(nullptr, 0);
+            auto cuts = [&](int at) { return (at & 15) && at > s0 && at < s0 + TILE; };
+            if (!cuts(see.n) && !cuts(see.win_begin) && !cuts(see.sink_end)) {
+                v_done(g);
+            } else {
+                due = true;
+                due_g = g;
+                due_s0 = s0;
+                due_see = see;
             }
         }
+        if (ok) wait_for(nullptr, 0);
         asm volatile("cp.async.wait_all;" ::: "memory");
         if (*(volatile int *)&sm.abort) {  // copies in flight land before the CTA leaves
-            for (int k = max(0, j - NSLOT); k < j; k++) {
-                const uint32_t addr = smem_u32(&sm.full[k % NSLOT]);
-                for (int it = 0; it < (1 << 20); it++) {
-                    uint32_t ok2;
-                    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-                                 : "=r"(ok2) : "r"(addr), "r"((uint32_t)((k / NSLOT) & 1)) : "memory");
-                    if (ok2) break;
-                }
-            }
+            for (int k = max(0, j - slots); k < j; k++)
+                bar_drain(&sm.full[ring0 + k % slots], (k / slots) & 1);
         }
     } else if (warp == 1) {
-        // ---- MMAs: S(gs) chunk by chunk as K lands, O(go) half by half as P and V are there,
-        // S at most one tile ahead: a ring slot's loads are then waited for in order
+        // ---- S(g) = K(g) Q^T, as the softmax frees its buffer and K lands --------------------
         if (lane == 0) {
-            const uint32_t id1 = idesc_bf16(128, N, false, false);
-            const uint32_t id2 = idesc_bf16(128, N, true, false);
-            const uint32_t ring0 = smem_u32(sm.ring[0]);
+            const uint32_t id = idesc_bf16(128, N, false, false);
+            const uint64_t dk0 = sdesc_sw128(smem_u32(sm.ring[0]), 16, 1024);
+            const uint64_t dq0 = sdesc_sw128(smem_u32(sm.q[0][0]), 16, 1024);
+            bool ok = true;
+            int g = 0, kq = 0, sl = 0;
+            uint32_t phase = 0;
             Walk w = start;
-            w.skip_empty();
-            int left = w.done() ? 0 : w.cnt;  // S tiles to go in the item
-            bool first = true;                // the item's first S: q must be there
-            int kq = 0, gs = 0, cs = 0, go = 0, ho = 0;
-            bool s_started = false, o_started = false, ok = true;
-            uint32_t spins = 0;
-            uint64_t t_idle = 0;
-            while (ok && (left > 0 || go < gs)) {
-                bool progressed = false;
-                if (go < gs) {
-                    const int bb = go & 1;
-                    if (!o_started && bar_test(&sm.p_full[bb], (go >> 1) & 1) &&
-                        (go < 2 || bar_test(&sm.o_empty[bb], ((go >> 1) - 1) & 1)))
-                        o_started = true;
-                    if (o_started) {
-                        const int j0 = 8 * go + 4 + 2 * ho, s0 = j0 % NSLOT, s1 = s0 + 1;
-                        if (bar_test(&sm.full[s0], (j0 / NSLOT) & 1) &&
-                            bar_test(&sm.full[s1], ((j0 + 1) / NSLOT) & 1)) {
-                            tc_fence_after();
-                            const uint32_t pb = smem_u32(sm.p[bb][0]);
+                for (; !w.done() && ok; w.next(), kq++) {
+                const uint64_t dq = sdesc_add(dq0, (kq % QB) * (uint32_t)sizeof(sm.q[0]));
+                ok = bar_wait(&sm.q_full[kq % QB], (kq / QB) & 1, &sm.abort, status, VX_DEV_TIMEOUT_MMA);
+                for (int i = 0; i < w.cnt && ok; i++, g++) {
+                    const int bb = g & 1;
+                    if (g >= 2)
+                        ok = bar_wait(&sm.s_empty[bb], ((g >> 1) - 1) & 1, &sm.abort, status,
+                                      VX_DEV_TIMEOUT_MMA);
+                    for (int c = 0; c < 4 && ok; c++) {
+                        ok = bar_wait(&sm.full[sl], phase, &sm.abort, status, VX_DEV_TIMEOUT_TMA);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint64_t dk = sdesc_add(dk0, sl * CHUNK);
+                        const uint64_t dqc = sdesc_add(dq, c * (Sm::ROWS * 128));
 #pragma unroll
-                            for (int kk = 0; kk < 8; kk++)
-                                mma_bf16(tmem + TM_O + (bb * 2 + ho) * N,
-                                         sdesc_sw128(ring0 + s0 * CHUNK + kk * 2048, CHUNK, 1024),
-                                         sdesc_sw128(pb + (kk >> 2) * (Sm::ROWS * 128) + (kk & 3) * 32,
-                                                     16, 1024),
-                                         id2, kk != 0);
-                            mma_commit(&sm.empty[s0]);
-                            mma_commit(&sm.empty[s1]);
-                            progressed = true;
-                            if (++ho == 2) {
-                                mma_commit(&sm.o_full[bb]);
-                                ho = 0;
-                                o_started = false;
-                                go++;
-                            }
+                        for (int kk = 0; kk < 4; kk++)
+                            mma_bf16(tmem + bb * N, sdesc_add(dk, kk * 32), sdesc_add(dqc, kk * 32), id,
+                                     (c | kk) != 0);
+                        mma_commit(&sm.empty[sl]);
+                        if (++sl == NK) {
+                            sl = 0;
+                            phase ^= 1;
                         }
                     }
+                    if (ok) mma_commit(&sm.s_full[bb]);
                 }
-                if (left > 0 && gs - go <= 1) {
-                    const int bb = gs & 1;
-                    if (!s_started && (!first || bar_test(&sm.q_full[kq % QB], (kq / QB) & 1)) &&
-                        (gs < 2 || bar_test(&sm.s_empty[bb], ((gs >> 1) - 1) & 1)))
-                        s_started = true;
-                    if (s_started) {
-                        const int j = 8 * gs + cs, slot = j % NSLOT;
-                        if (bar_test(&sm.full[slot], (j / NSLOT) & 1)) {
-                            tc_fence_after();
-                            const uint32_t q0 = smem_u32(sm.q[kq % QB][0]);
-#pragma unroll
-                            for (int kk = 0; kk < 4; kk++)
-                                mma_bf16(tmem + bb * N,
-                                         sdesc_sw128(ring0 + slot * CHUNK + kk * 32, 16, 1024),
-                                         sdesc_sw128(q0 + cs * (Sm::ROWS * 128) + kk * 32, 16, 1024),
-                                         id1, (cs | kk) != 0);
-                            mma_commit(&sm.empty[slot]);
-                            progressed = true;
-                            first = false;
-                            if (++cs == 4) {
-                                mma_commit(&sm.s_full[bb]);
-                                cs = 0;
-                                s_started = false;
-                                gs++;
-                                if (--left == 0) {  // the item's S MMAs are all issued
-                                    mma_commit(&sm.q_empty[kq % QB]);
-                                    kq++;
-                                    first = true;
-                                    w.next_work();
-                                    left = w.done() ? 0 : w.cnt;
-                                }
-                            }
+                if (ok) mma_commit(&sm.q_empty[kq % QB]);
+            }
+            mma_commit(&sm.mma_done[0]);
+            bar_drain(&sm.mma_done[0], 0);  // also after an abort
+        }
+    } else if (warp == O_WARP) {
+        // ---- O(g) = V(g)^T P(g)^T, half by half as P is written and V lands -------------------
+        if (lane == 0) {
+            const uint32_t id = idesc_bf16(128, N, true, false);
+            const uint64_t dv0 = sdesc_sw128(smem_u32(sm.ring[NK]), CHUNK, 1024);
+            const uint64_t dp0 = sdesc_sw128(smem_u32(sm.p[0][0]), 16, 1024);
+            bool ok = true;
+            int g = 0, sl = 0;
+            uint32_t phase = 0;
+            Walk w = start;
+                for (; !w.done() && ok; w.next()) {
+                for (int i = 0; i < w.cnt && ok; i++, g++) {
+                    const int bb = g & 1;
+                    const uint32_t seen = w.t.seen_groups(w.t.first_slot(w.v0 + i));
+                    const uint64_t dp = sdesc_add(dp0, bb * (uint32_t)sizeof(sm.p[0]));
+                    if (g >= 2)
+                        ok = bar_wait(&sm.o_empty[bb], ((g >> 1) - 1) & 1, &sm.abort, status,
+                                      VX_DEV_TIMEOUT_MMA);
+                    ok = ok && bar_wait(&sm.p_full[bb], (g >> 1) & 1, &sm.abort, status, VX_DEV_TIMEOUT_MMA);
+                    ok = ok && bar_wait(&sm.v_ok[bb], (g >> 1) & 1, &sm.abort, status, VX_DEV_TIMEOUT_TMA);
+                    for (int ho = 0; ho < 2 && ok; ho++) {
+                        ok = bar_wait(&sm.full[NK + sl], phase, &sm.abort, status, VX_DEV_TIMEOUT_TMA) &&
+                             bar_wait(&sm.full[NK + sl + 1], phase, &sm.abort, status, VX_DEV_TIMEOUT_TMA);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint64_t dv = sdesc_add(dv0, sl * CHUNK);
+                        const uint32_t d = tmem + TM_O + (bb * 2 + ho) * N;
+                        uint32_t acc = 0;
+#pragma unroll 2
+                        for (int kk = 0; kk < 8; kk++) {  // the 16-slot groups with a seen slot
+                            if (!((seen >> kk) & 1)) continue;
+                            mma_bf16(d, sdesc_add(dv, kk * 2048),
+                                     sdesc_add(dp, (kk >> 2) * (Sm::ROWS * 128) + (kk & 3) * 32), id, acc);
+                            acc = 1;
+                        }
+                        mma_commit(&sm.empty[NK + sl]);
+                        mma_commit(&sm.empty[NK + sl + 1]);
+                        if ((sl += 2) == NV) {
+                            sl = 0;
+                            phase ^= 1;
                         }
                     }
-                }
-                if (progressed) {
-                    spins = 0;
-                } else if ((++spins & 255) == 0) {  // bounded like every wait
-                    if (*(volatile int *)&sm.abort) ok = false;
-                    const uint64_t now = now_ns();
-                    if (spins == 256) t_idle = now;
-                    else if (now - t_idle > 2000000000ull) {
-                        *(volatile int *)&sm.abort = 1;
-                        dev_flag(status, VX_DEV_TIMEOUT_MMA);
-                        ok = false;
-                    }
+                    if (ok) mma_commit(&sm.o_full[bb]);
                 }
             }
-            mma_commit(&sm.mma_done);
-            for (int it = 0; it < (1 << 20); it++)  // also after an abort
-                if (bar_test(&sm.mma_done, 0)) break;
+            mma_commit(&sm.mma_done[1]);
+            bar_drain(&sm.mma_done[1], 0);
         }
-    } else if (warp < 6) {
+    } else if (warp < STAGE_WARP) {
         // ---- softmax: thread = slot r of the tile; then output dims r and r + 128 ----------
         const int q4 = warp & 3, r = q4 * 32 + lane;
         const uint32_t lane_addr = tmem + ((uint32_t)(q4 * 32) << 16);
         const float sc2 = 1.4426950408889634f * 0.0625f;  // log2(e) / sqrt(256)
         bool ok = true;
         int g = 0, kq = 0;  // tiles and items so far
-        Walk w = start;
-        w.skip_empty();
-        for (; !w.done() && ok; w.next_work()) {
-            float m2[G], l[G], acc_a[G], acc_b[G], al[G], al_prev[G];
+        float m2[G], l[G], acc_a[G], acc_b[G], al[G], al_prev[G];
+        auto reset = [&]() {
 #pragma unroll
             for (int h = 0; h < G; h++) {
                 m2[h] = -INFINITY;
-                l[h] = acc_a[h] = acc_b[h] = al[h] = al_prev[h] = 0.f;
+                l[h] = 0.f;
             }
-            auto fold = [&](int t) {  // O(t), with the rescale of its tile
-                const int bb = t & 1;
-                ok = ok && bar_wait(&sm.o_full[bb], (t >> 1) & 1, &sm.abort, status,
-                                    VX_DEV_TIMEOUT_MMA);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) return;
-                tc_fence_after();
-                float oa[N], ob[N];
-                tmem_ld_cols(lane_addr + TM_O + bb * 2 * N, oa);
-                tmem_ld_cols(lane_addr + TM_O + (bb * 2 + 1) * N, ob);
-                tc_fence_before();
-                mbar_arrive(&sm.o_empty[bb]);
+        };
+#pragma unroll
+        for (int h = 0; h < G; h++) acc_a[h] = acc_b[h] = al[h] = al_prev[h] = 0.f;
+        reset();
+        auto fold = [&](int t) {  // O(t), with the rescale of its tile
+            const int bb = t & 1;
+            ok = ok && bar_wait(&sm.o_full[bb], (t >> 1) & 1, &sm.abort, status, VX_DEV_TIMEOUT_MMA);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) return;
+            tc_fence_after();
+            auto half = [&](int ho, float (&acc)[G]) {
+                float o[N];
+                tmem_ld_cols(lane_addr + TM_O + (bb * 2 + ho) * N, o);
 #pragma unroll
                 for (int h = 0; h < G; h++) {
-                    float xa = oa[h + (TERMS - 1) * G], xb = ob[h + (TERMS - 1) * G];
+                    float x = o[h + (TERMS - 1) * G];
 #pragma unroll
-                    for (int k = TERMS - 2; k >= 0; k--) {  // small terms first
-                        xa += oa[h + k * G];
-                        xb += ob[h + k * G];
-                    }
-                    acc_a[h] = fmaf(acc_a[h], al_prev[h], xa);
-                    acc_b[h] = fmaf(acc_b[h], al_prev[h], xb);
+                    for (int k = TERMS - 2; k >= 0; k--) x += o[h + k * G];  // small terms first
+                    acc[h] = fmaf(acc[h], al_prev[h], x);
                 }
             };
+            half(0, acc_a);
+            half(1, acc_b);
+            tc_fence_before();
+            mbar_arrive(&sm.o_empty[bb]);
+        };
+        // An item ends in two steps: its sums and maxima go to shared memory (close) before the
+        // next item's first tile uses the registers, its rows to the output buffer (finish)
+        // after that tile's P is written: the wait for the last O does not hold the next S up.
+        auto close = [&](int k) {
+            const int eb = k & 1;
+#pragma unroll
+            for (int h = 0; h < G; h++) {
+                const float t = warp_sum(l[h]);
+                if (lane == 0) sm.red_sum[eb][q4][h] = t;
+                if (r == 0) sm.m_fin[eb][h] = m2[h];
+            }
+            mbar_arrive(&sm.grp_end[eb]);
+            reset();
+        };
+        auto finish = [&](int k) {
+            const int eb = k & 1;
+            ok = bar_wait(&sm.grp_end[eb], (k >> 1) & 1, &sm.abort, status, VX_DEV_TIMEOUT_MMA) && ok;
+            if (k > 0)
+                ok = bar_wait(&sm.ob_empty, (k - 1) & 1, &sm.abort, status, VX_DEV_TIMEOUT_MMA) && ok;
+            ok = __all_sync(0xffffffffu, ok);
+#pragma unroll
+            for (int h = 0; h < G; h++) {
+                const float L = sm.red_sum[eb][0][h] + sm.red_sum[eb][1][h] +
+                                sm.red_sum[eb][2][h] + sm.red_sum[eb][3][h];
+                const float inv = 1.0f / L;
+                sm.ob[h][r] = acc_a[h] * inv;
+                sm.ob[h][r + 128] = acc_b[h] * inv;
+                acc_a[h] = acc_b[h] = 0.f;
+                if (r == 0) {
+                    sm.ml[h][0] = sm.m_fin[eb][h];
+                    sm.ml[h][1] = L;
+                }
+            }
+            mbar_arrive(&sm.ob_full);
+        };
+        Walk w = start;
+        for (; !w.done() && ok; w.next(), kq++) {
             float *sc = nullptr;  // the item's scores [G][slots], for the weight sums
             if constexpr (TERMS == 3)
                 if (a.scores)
                     sc = a.scores + (size_t)(w.b * nkv + w.h) * G * a.score_stride;
-            for (int i = 0; i < w.cnt && ok; i++) {
-                const int gi = g + i, bb = gi & 1;
-                ok = bar_wait(&sm.s_full[bb], (gi >> 1) & 1, &sm.abort, status, VX_DEV_TIMEOUT_MMA);
+            for (int i = 0; i < w.cnt && ok; i++, g++) {
+                const int bb = g & 1;
+                if (i == 0 && kq > 0) close(kq - 1);
+                ok = bar_wait(&sm.s_full[bb], (g >> 1) & 1, &sm.abort, status, VX_DEV_TIMEOUT_MMA);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_fence_after();
@@ -528,11 +641,13 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
 #pragma unroll
                     for (int k = TERMS - 2; k >= 0; k--) t += s[h + k * G];
                     x[h] = valid ? t * sc2 : -INFINITY;
+                    if constexpr (TERMS == 3)
+                        if (sc && valid) sc[(size_t)h * a.score_stride + (w.v0 + i) * TILE + r] = x[h];
                     t = warp_max_redux(x[h]);
                     if (lane == 0) sm.red_max[bb][q4][h] = t;
                 }
                 mbar_arrive(&sm.grp[bb]);  // all four warps' maxima
-                ok = bar_wait(&sm.grp[bb], (gi >> 1) & 1, &sm.abort, status, VX_DEV_TIMEOUT_MMA);
+                ok = bar_wait(&sm.grp[bb], (g >> 1) & 1, &sm.abort, status, VX_DEV_TIMEOUT_MMA);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 uint8_t *pbuf = sm.p[bb][r >> 6];
@@ -541,74 +656,37 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
                     const float t = fmaxf(fmaxf(sm.red_max[bb][0][h], sm.red_max[bb][1][h]),
                                           fmaxf(sm.red_max[bb][2][h], sm.red_max[bb][3][h]));
                     const float mn = fmaxf(m2[h], t);
-                    al[h] = exp2f(m2[h] - mn);
+                    al[h] = ex2_approx(m2[h] - mn);
                     m2[h] = mn;
-                    float p = exp2f(x[h] - mn);
-                    l[h] = fmaf(l[h], al[h], p);
-#pragma unroll
-                    for (int k = 0; k < TERMS; k++) {
-                        const uint16_t t16 = f32_to_bf16(p);
-                        *reinterpret_cast<uint16_t *>(pbuf + sw128(h + k * G, r & 63)) = t16;
-                        p -= bf16_to_f32(t16);
-                    }
+                    x[h] = ex2_approx(x[h] - mn);
+                    l[h] = fmaf(l[h], al[h], x[h]);
                 }
-                // a tile with unseen slots: their V rows may hold anything (or not have been
-                // copied), and 0 * NaN is NaN, so they are zeroed before V^T P^T reads them. The
-                // previous O is folded first: the ring slot's load before this one has then
-                // been waited for
-                const bool part = s0 + TILE > w.t.see.n ||
-                                  (s0 < w.t.see.win_begin && s0 + TILE > w.t.see.sink_end);
-                if (part) {
-                    if (i >= 1) fold(gi - 1);
-                    for (int k = 0; k < 4 && ok; k++) {
-                        const int j = 8 * gi + 4 + k;
-                        ok = bar_wait(&sm.full[j % NSLOT], (j / NSLOT) & 1, &sm.abort, status,
-                                      VX_DEV_TIMEOUT_TMA);
-                        if (ok && !valid) {
-                            uint4 *row = reinterpret_cast<uint4 *>(sm.ring[j % NSLOT] + r * 128);
 #pragma unroll
-                            for (int e = 0; e < 8; e++) row[e] = make_uint4(0, 0, 0, 0);
+                for (int k = 0; k < TERMS; k++)
+#pragma unroll
+                    for (int h = 0; h < G; h += 2) {  // two heads per conversion
+                        const int h1 = h + 1 < G ? h + 1 : h;
+                        const uint32_t t = pack_bf16x2(x[h], x[h1]);
+                        *reinterpret_cast<uint16_t *>(pbuf + sw128(h + k * G, r & 63)) = (uint16_t)t;
+                        x[h] -= bf16_to_f32(t & 0xffffu);
+                        if (h1 > h) {
+                            *reinterpret_cast<uint16_t *>(pbuf + sw128(h1 + k * G, r & 63)) =
+                                (uint16_t)(t >> 16);
+                            x[h1] -= __uint_as_float(t & 0xffff0000u);
                         }
                     }
-                }
                 fence_proxy_async();
                 mbar_arrive(&sm.p_full[bb]);
-                if (i >= 1 && !part) fold(gi - 1);
+                if (g > 0) fold(g - 1);
+                if (i == 0 && kq > 0) finish(kq - 1);
 #pragma unroll
                 for (int h = 0; h < G; h++) al_prev[h] = al[h];
-                if constexpr (TERMS == 3)
-                    if (sc && valid)
-#pragma unroll
-                        for (int h = 0; h < G; h++)
-                            sc[(size_t)h * a.score_stride + (w.v0 + i) * TILE + r] = x[h];
             }
-            if (ok) fold(g + w.cnt - 1);
-            const int eb = kq & 1;
-#pragma unroll
-            for (int h = 0; h < G; h++) {
-                const float t = warp_sum(l[h]);
-                if (lane == 0) sm.red_sum[eb][q4][h] = t;
-            }
-            mbar_arrive(&sm.grp_end[eb]);
-            ok = bar_wait(&sm.grp_end[eb], (kq >> 1) & 1, &sm.abort, status, VX_DEV_TIMEOUT_MMA) && ok;
-            if (kq > 0)
-                ok = bar_wait(&sm.ob_empty, (kq - 1) & 1, &sm.abort, status, VX_DEV_TIMEOUT_MMA) && ok;
-            ok = __all_sync(0xffffffffu, ok);
-#pragma unroll
-            for (int h = 0; h < G; h++) {
-                const float L = sm.red_sum[eb][0][h] + sm.red_sum[eb][1][h] +
-                                sm.red_sum[eb][2][h] + sm.red_sum[eb][3][h];
-                const float inv = 1.0f / L;
-                sm.ob[h][r] = acc_a[h] * inv;
-                sm.ob[h][r + 128] = acc_b[h] * inv;
-                if (r == 0) {
-                    sm.ml[h][0] = m2[h];
-                    sm.ml[h][1] = L;
-                }
-            }
-            mbar_arrive(&sm.ob_full);
-            g += w.cnt;
-            kq++;
+        }
+        if (kq > 0 && ok) {
+            close(kq - 1);
+            fold(g - 1);
+            finish(kq - 1);
         }
     } else {
         // ---- q in, results out --------------------------------------------------------------
@@ -641,23 +719,13 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
             mbar_arrive(&sm.q_full[qb]);
         };
         Walk nx = start;  // the item whose q is staged next
-        nx.skip_empty();
         if (!nx.done()) {
             load_q(nx);
             store_q(0);
-            nx.next_work();
+            nx.next();
         }
         for (Walk w = start; !w.done() && ok; w.next()) {
             const size_t base = ((size_t)w.b * a.nq + w.h * G) * HD + d0;
-            if (w.empty()) {
-#pragma unroll
-                for (int h = 0; h < G; h++) {
-                    const float z[8] = {};
-                    if (a.out_bf16) st8_bf16(static_cast<uint16_t *>(a.out) + base + h * HD, z);
-                    else st8_f32(static_cast<float *>(a.out) + base + h * HD, z);
-                }
-                continue;
-            }
             if (!nx.done()) {
                 load_q(nx);
                 // the S MMAs of the item that used the buffer before are complete
@@ -666,7 +734,7 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
                                   status, VX_DEV_TIMEOUT_MMA);
                 ok = __all_sync(0xffffffffu, ok);
                 if (ok) store_q((kq + 1) % QB);
-                nx.next_work();
+                nx.next();
             }
             const bool whole = w.whole();
             float gv[G][8];
@@ -680,32 +748,37 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
             ok = ok && bar_wait(&sm.ob_full, kq & 1, &sm.abort, status, VX_DEV_TIMEOUT_MMA);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
+            // the buffer is free once it is in registers (an arrival after the global stores
+            // waits for them)
+            float o[G][8];
+#pragma unroll
+            for (int h = 0; h < G; h++) ld8_f32(o[h], &sm.ob[h][d0]);
+            const float2 ml = lane < G ? make_float2(sm.ml[lane][0], sm.ml[lane][1]) : make_float2(0, 0);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.ob_empty);
             const size_t rec = (size_t)(2 * c + (w.v0 > 0 ? 0 : 1)) * G;
+            const int item = w.b * nkv + w.h;
 #pragma unroll
             for (int h = 0; h < G; h++) {
-                float o[8];
-                ld8_f32(o, &sm.ob[h][d0]);
                 if (!whole) {
-                    st8_f32(a.rec_o + (rec + h) * HD + d0, o);
+                    st8_f32(a.rec_o + (rec + h) * HD + d0, o[h]);
                 } else {
                     if (a.gate)
 #pragma unroll
-                        for (int e = 0; e < 8; e++) o[e] *= 1.0f / (1.0f + expf(-gv[h][e]));
-                    if (a.out_bf16) st8_bf16(static_cast<uint16_t *>(a.out) + base + h * HD, o);
-                    else st8_f32(static_cast<float *>(a.out) + base + h * HD, o);
+                        for (int e = 0; e < 8; e++)
+                            o[h][e] *= TERMS == 2 ? __fdividef(1.0f, 1.0f + __expf(-gv[h][e]))
+                                                  : 1.0f / (1.0f + expf(-gv[h][e]));
+                    if (a.out_bf16) st8_bf16(static_cast<uint16_t *>(a.out) + base + h * HD, o[h]);
+                    else st8_f32(static_cast<float *>(a.out) + base + h * HD, o[h]);
                 }
             }
-            const int item = w.b * nkv + w.h;
             if (lane < G) {
-                const float2 ml = make_float2(sm.ml[lane][0], sm.ml[lane][1]);
                 if (!whole) a.rec_ml[rec + lane] = ml;
                 else if (a.scores) a.item_ml[(size_t)item * G + lane] = ml;
             }
             // which runs hold the item, for the weight sums
             if (lane == 0 && a.scores && w.v0 == 0)
-                a.span[item] = make_int2(c, owner(w.u + w.t.units() - 1));
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.ob_empty);
+                a.span[item] = make_int2(c, owner(end - w.left + w.t.tiles - 1));
             kq++;
         }
     }
@@ -718,7 +791,7 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
 }
 
 // ---- join and weight sums ---------------------------------------------------------------
-// Blocks [0, (P - 1) G): block (c, h) merges head h of the item that run c continues, if c is
+// Blocks [0, B): zeros for a sequence without slots. Then (P - 1) G blocks: (c, h) merges head h of the item that run c continues, if c is
 // the second run of it: o = sum_r w_r o_r / sum_r w_r, w_r = l_r 2^(m_r - m). The other blocks
 // add the weights of 256 slots of an item: sum_h 2^(s_h - m_h) / l_h.
 __global__ void __launch_bounds__(256)
@@ -726,7 +799,16 @@ paged_join_k(const __grid_constant__ DecodeArgs a, int P, int G, int slot_blocks
     grid_dep_wait();
     __shared__ float w_s[JOIN_MAX], red[8];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int n_join = (P - 1) * G;
+    const int n_join = (P - 1) * G, blk = (int)blockIdx.x - a.B;
+    if (blk < 0) {
+        if (a.lens[blockIdx.x] > 0) return;
+        for (int i = tid; i < a.nq * HD; i += 256) {
+            const size_t at = (size_t)blockIdx.x * a.nq * HD + i;
+            if (a.out_bf16) act_st<true>(a.out, at, 0.f);
+            else act_st<false>(a.out, at, 0.f);
+        }
+        return;
+    }
     // records of runs c1 .. c2: the first is that run's last item, the others first items
     auto rec_of = [](int c1, int r) { return (size_t)(r == 0 ? 2 * c1 + 1 : 2 * (c1 + r)); };
     auto block_max = [&](float m) {
@@ -738,9 +820,9 @@ paged_join_k(const __grid_constant__ DecodeArgs a, int P, int G, int slot_blocks
         for (int i = 1; i < 8; i++) t = fmaxf(t, red[i]);
         return t;
     };
-    if ((int)blockIdx.x < n_join) {
-        const int4 j = a.join[blockIdx.x / G + 1];
-        const int h = blockIdx.x % G;
+    if (blk < n_join) {
+        const int4 j = a.join[blk / G + 1];
+        const int h = blk % G;
         if (j.x < 0) return;
         const int c1 = j.y, n = j.z - j.y + 1;
         float m = -INFINITY;
@@ -774,9 +856,9 @@ paged_join_k(const __grid_constant__ DecodeArgs a, int P, int G, int slot_blocks
         else act_st<false>(a.out, i, o);
         return;
     }
-    const int bi = blockIdx.x - n_join, item = bi / slot_blocks;
+    const int bi = blk - n_join, item = bi / slot_blocks;
     const int b = item / a.pool.nkv, k = (bi % slot_blocks) * 256 + tid;
-    const SeqTiles t = Walk::seq(a, b);
+    const SeqTiles t(seq_len(a, b), a.window, a.sinks);
     if ((bi % slot_blocks) * 256 >= t.tiles * TILE) return;
     const int2 span = a.span[item];
     const int n = span.y - span.x + 1;
@@ -856,7 +938,7 @@ int launch_paged_decode(const DecodeArgs &a, const void *k_pages, const void *v_
         return -1;
     const int G = a.nq / a.pool.nkv;
     const int slot_blocks = a.scores ? (int)((a.score_stride + 255) / 256) : 0;
-    const long long blocks = (long long)(P - 1) * G + (long long)slot_blocks * a.B * a.pool.nkv;
+    const long long blocks = a.B + (long long)(P - 1) * G + (long long)slot_blocks * a.B * a.pool.nkv;
     if (blocks > 0x7fffffffLL)
         return fail(err, errlen, "vx27_gqa_paged_decode: weight sums over %d sequences of %zu slots",
                     a.B, a.score_stride);
@@ -877,8 +959,7 @@ int launch_paged_decode(const DecodeArgs &a, const void *k_pages, const void *v_
     }
 #undef VX_G
 #undef VX_D
-    if (blocks > 0)
-        VX_CK(launch_pdl(paged_join_k, dim3((unsigned)blocks), dim3(256), 0, st, a, P, G, slot_blocks));
+    VX_CK(launch_pdl(paged_join_k, dim3((unsigned)blocks), dim3(256), 0, st, a, P, G, slot_blocks));
     return 0;
 }
 
