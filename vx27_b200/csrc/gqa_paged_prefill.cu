@@ -99,21 +99,20 @@ struct Sync {
         dev_flag(status, code);
     }
     __device__ bool aborted() const { return *(volatile int *)abort != 0; }
-    __device__ bool wait(uint64_t *bar, uint32_t parity, uint32_t code) const {
-        const uint32_t addr = smem_u32(bar);
-        uint64_t t0 = 0;
-        for (uint32_t it = 0;; ++it) {
+    // only the first try is inlined: the roles' loops share the instruction cache
+    __device__ __noinline__ bool wait_long(uint32_t addr, uint32_t parity, uint32_t code) const {
+        const uint64_t t0 = now_ns();
+        for (;;) {
             if (try_wait(addr, parity)) return true;
-            if ((it & 255) == 0) {
-                if (aborted()) return false;
-                const uint64_t now = now_ns();
-                if (it == 0) t0 = now;
-                else if (now - t0 > 2000000000ull) {
-                    fail(code);
-                    return false;
-                }
-            }
+            if (aborted()) return false;
+            if (now_ns() - t0 > 2000000000ull) break;
         }
+        fail(code);
+        return false;
+    }
+    __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, uint32_t code) const {
+        const uint32_t addr = smem_u32(bar);
+        return try_wait(addr, parity) || wait_long(addr, parity, code);
     }
     // a softmax warp's arrival on rank 0's barrier (16 of the pair's)
     __device__ void arrive(uint64_t *bar) const {
@@ -237,16 +236,19 @@ __device__ __forceinline__ void softmax_role(Smem &sm, const Sync &sy, const Pro
     sm.xsum[hf][r] = l_run;
     named_bar_sync(1, 256);
     const float l_row = l_run + sm.xsum[hf ^ 1][r];
-    // the gate is requested before O is final; its sigmoid uses the SFU's 2^x and reciprocal
+    // the result by 32 columns, in a loop that is not unrolled (its code is shared by all of
+    // the row's columns), the gate requested one round ahead; its sigmoid uses the SFU's 2^x
+    // and reciprocal
     const int t_row = t0 + r;
     const size_t base = ((size_t)t_row * a.nq + h) * HD + hf * (HD / 2);
-    uint4 graw[HD / 16];
     const bool gated = a.gate && t_row < a.T;
-    if (gated) {
-        const uint4 *gp = reinterpret_cast<const uint4 *>(a.gate + base);
+    uint4 gate[4], next[4];
+    auto request = [&](int i) {
+        const uint4 *gp = reinterpret_cast<const uint4 *>(a.gate + base) + 4 * i;
 #pragma unroll
-        for (int k = 0; k < HD / 16; k++) graw[k] = gp[k];
-    }
+        for (int k = 0; k < 4; k++) next[k] = gp[k];
+    };
+    if (gated) request(0);
     if (ok) ok = sy.wait(&sm.o_final, 0, VX_DEV_TIMEOUT_MMA);
     ok = __all_sync(0xffffffffu, ok);
     if (!ok) {
@@ -255,26 +257,29 @@ __device__ __forceinline__ void softmax_role(Smem &sm, const Sync &sy, const Pro
     }
     tc_fence_after();
     const float inv = 1.0f / l_row;
-#pragma unroll
-    for (int i = 0; i < HD / 128; i++) {
-        float o[64];
-        tmem_ld64(tO + lane_off + hf * (HD / 2) + 64 * i, o);
+#pragma unroll 1
+    for (int i = 0; i < HD / 64; i++) {
+        float o[32];
+        tmem_ld16(tO + lane_off + hf * (HD / 2) + 32 * i, o);
+        tmem_ld16(tO + lane_off + hf * (HD / 2) + 32 * i + 16, o + 16);
         if (t_row >= a.T) continue;
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
+        for (int k = 0; k < 4; k++) gate[k] = next[k];
+        if (gated && i < HD / 64 - 1) request(i + 1);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
             float x[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) x[e] = o[8 * k + e] * inv;
             if (gated) {
-                const uint4 gv = graw[8 * i + k];
-                const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w};
+                const uint32_t gw[4] = {gate[k].x, gate[k].y, gate[k].z, gate[k].w};
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     x[2 * e] *= __fdividef(1.0f, 1.0f + __expf(-bf16_to_f32(gw[e] & 0xffffu)));
                     x[2 * e + 1] *= __fdividef(1.0f, 1.0f + __expf(-bf16_to_f32(gw[e] >> 16)));
                 }
             }
-            st8_bf16(a.out + base + 64 * i + 8 * k, x);
+            st8_bf16(a.out + base + 32 * i + 8 * k, x);
         }
     }
 }
