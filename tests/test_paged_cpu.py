@@ -123,7 +123,7 @@ def test_wrapper_refusals():
             (dict(k_in=kv.float()), "k_in: dtype"), (dict(v_in=kv[:, :2]), "v_in: shape"),
             (dict(pos=i(n + 1)), "pos: shape"), (dict(seq=i(n).long()), "seq: dtype"),
             (dict(q_out=x.half()), "q_out: dtype"), (dict(rope=torch.zeros(64)), "rope: shape"),
-            (dict(q_norm_w=torch.zeros(8)), "q_norm_w: 8 elements"),
+            (dict(q_norm_w=torch.zeros(8)), "q_norm_w: shape"),
             (dict(page_table=i(mp)), "page_table: shape")]:
         with pytest.raises(E, match=message):
             app(**change)

@@ -86,7 +86,11 @@ __device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, int *ab
     const uint32_t addr = smem_u32(bar);
     return bar_try(addr, parity) || bar_wait_long(addr, parity, abort, status, code);
 }
-__device__ __noinline__ int mul_div(int a, int b, int c) { return (int)((long long)a * b / c); }
+// (a b + add) / c, a quotient that fits 32 bits.
+__device__ __noinline__ int mul_div(int a, int b, int c, int add = 0) {
+    const unsigned long long x = (unsigned long long)a * b + add;
+    return (int)(x >> 32 ? x / c : (unsigned)x / (unsigned)c);
+}
 // Bounded wait that goes on after an abort: what must be done before the CTA may leave.
 __device__ __forceinline__ void bar_drain(uint64_t *bar, uint32_t parity) {
     for (int it = 0; it < (1 << 20); it++)
@@ -279,11 +283,12 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
     // ---- the run of this CTA: tiles [c T / P, (c + 1) T / P) of the T in all ------------
     const int cb = (a.B + THREADS - 1) / THREADS;  // consecutive sequences per thread
     const int b_lo = min(tid * cb, a.B), b_hi = min(b_lo + cb, a.B);
-    int mine = 0;
+    int mine = 0, n0 = 0;  // tiles of the thread's sequences; the first one's length
     for (int b = b_lo; b < b_hi; b++) {
-        const int n = a.lens[b];
-        if (n < 0 || n > a.max_pages << a.pool.ps_log) dev_flag(status, VX_DEV_BAD_ARG);
-        mine += SeqTiles(seq_len(a, b), a.window, a.sinks).tiles * nkv;
+        const int n = a.lens[b], nc = min(max(n, 0), a.max_pages << a.pool.ps_log);
+        if (n != nc) dev_flag(status, VX_DEV_BAD_ARG);
+        if (b == b_lo) n0 = nc;
+        mine += SeqTiles(nc, a.window, a.sinks).tiles * nkv;
     }
     int incl = mine;
 #pragma unroll
@@ -302,7 +307,7 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
     const int begin = c < P ? mul_div(c, total, P) : 0, end = c < P ? mul_div(c + 1, total, P) : 0;
     if (begin < end && begin >= before && begin < before + mine) {
         int b = b_lo, at = before;
-        for (;; b++) {
+        for (; cb > 1; b++) {
             const int k = SeqTiles(seq_len(a, b), a.window, a.sinks).tiles * nkv;
             if (begin < at + k) break;
             at += k;
@@ -315,21 +320,15 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
     tc_fence_after();
     const uint32_t tmem = sm.tmem_base;
     const int run_b = begin < end ? sm.run_b : 0;
-    if (tid < RUN_LENS && run_b + tid < a.B) sm.lens[tid] = seq_len(a, run_b + tid);
+    if (cb == 1) {  // thread b has the length of sequence b
+        if (tid >= run_b && tid < run_b + RUN_LENS) sm.lens[tid - run_b] = n0;
+    } else if (tid < RUN_LENS && run_b + tid < a.B) {
+        sm.lens[tid] = seq_len(a, run_b + tid);
+    }
     __syncthreads();
     const Walk start(a, sm.lens, run_b, begin < end ? sm.run_off : 0, end - begin);
     // the run that holds tile u
-    auto owner = [&](int u) { return (int)((((long long)u + 1) * P - 1) / total); };
-    // an item that began in an earlier run is joined by the block of its second run
-    if (tid == 0) {
-        int4 j = make_int4(-1, 0, 0, 0);
-        if (!start.done() && start.v0 > 0) {
-            const int s = begin - start.v0;
-            const int c1 = owner(s), c2 = owner(s + start.t.tiles - 1);
-            if (c == c1 + 1) j = make_int4(start.b * nkv + start.h, c1, c2, 0);
-        }
-        a.join[c] = j;
-    }
+    auto owner = [&](int u) { return mul_div(u + 1, P, total, -1); };
 
     if (warp == 0 || warp == V_WARP) {
         // ---- copies of K (warp 0) and of V: lane i < 8 has rows [16 i, 16 i + 16) of a tile ----
@@ -368,8 +367,10 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
             if (lane == 0) mbar_arrive(&sm.v_ok[g & 1]);
         };
         auto zero_edges = [&]() {
-            auto edge = [&](int at) {  // the group that slot `at` is in, unless it begins there
-                if ((at & 15) == 0 || at < due_s0 || at >= due_s0 + TILE) return;
+#pragma unroll 1
+            for (int e = 0; e < 3; e++) {  // the groups that n, the window or the sinks end in
+                const int at = e == 0 ? due_see.n : e == 1 ? due_see.win_begin : due_see.sink_end;
+                if ((at & 15) == 0 || at < due_s0 || at >= due_s0 + TILE) continue;
                 for (int i = lane >> 3; i < 16; i += 4) {
                     const int slot = (at & ~15) + i;
                     if (due_see.sees(slot)) continue;
@@ -379,10 +380,7 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
                                                    (slot - due_s0) * 128 + (lane & 7) * 16) =
                             make_uint4(0, 0, 0, 0);
                 }
-            };
-            edge(due_see.n);
-            edge(due_see.win_begin);
-            edge(due_see.sink_end);
+            }
             due = false;
             v_done(due_g);
         };
@@ -617,14 +615,11 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
             mbar_arrive(&sm.ob_full);
         };
         Walk w = start;
-        for (; !w.done() && ok; w.next(), kq++) {
-            float *sc = nullptr;  // the item's scores [G][slots], for the weight sums
-            if constexpr (TERMS == 3)
-                if (a.scores)
-                    sc = a.scores + (size_t)(w.b * nkv + w.h) * G * a.score_stride;
-            for (int i = 0; i < w.cnt && ok; i++, g++) {
-                const int bb = g & 1;
-                if (i == 0 && kq > 0) close(kq - 1);
+        for (int i = 0;;) {  // tile i of the item; after the last tile once more, to finish it
+            const bool last = w.done(), ended = i == 0 && g > 0;
+            const int bb = g & 1;
+            if (ended) close(kq - 1);
+            if (!last) {
                 ok = bar_wait(&sm.s_full[bb], (g >> 1) & 1, &sm.abort, status, VX_DEV_TIMEOUT_MMA);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
@@ -633,20 +628,24 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
                 tmem_ld_cols(lane_addr + bb * N, s);
                 tc_fence_before();
                 mbar_arrive(&sm.s_empty[bb]);
-                const int s0 = w.t.first_slot(w.v0 + i);
-                const bool valid = w.t.see.sees(s0 + r);
+                const bool valid = w.t.see.sees(w.t.first_slot(w.v0 + i) + r);
 #pragma unroll
                 for (int h = 0; h < G; h++) {
                     float t = s[h + (TERMS - 1) * G];
 #pragma unroll
                     for (int k = TERMS - 2; k >= 0; k--) t += s[h + k * G];
                     x[h] = valid ? t * sc2 : -INFINITY;
-                    if constexpr (TERMS == 3)
-                        if (sc && valid) sc[(size_t)h * a.score_stride + (w.v0 + i) * TILE + r] = x[h];
                     t = warp_max_redux(x[h]);
                     if (lane == 0) sm.red_max[bb][q4][h] = t;
                 }
                 mbar_arrive(&sm.grp[bb]);  // all four warps' maxima
+                if constexpr (TERMS == 3)
+                    if (a.scores && valid) {  // [G][slots] of the item, for the weight sums
+                        float *sc = a.scores + (size_t)(w.b * nkv + w.h) * G * a.score_stride +
+                                    (w.v0 + i) * TILE + r;
+#pragma unroll
+                        for (int h = 0; h < G; h++) sc[(size_t)h * a.score_stride] = x[h];
+                    }
                 ok = bar_wait(&sm.grp[bb], (g >> 1) & 1, &sm.abort, status, VX_DEV_TIMEOUT_MMA);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
@@ -677,19 +676,22 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
                     }
                 fence_proxy_async();
                 mbar_arrive(&sm.p_full[bb]);
-                if (g > 0) fold(g - 1);
-                if (i == 0 && kq > 0) finish(kq - 1);
-#pragma unroll
-                for (int h = 0; h < G; h++) al_prev[h] = al[h];
             }
-        }
-        if (kq > 0 && ok) {
-            close(kq - 1);
-            fold(g - 1);
-            finish(kq - 1);
+            if (g > 0) fold(g - 1);
+            if (ended) finish(kq - 1);
+            if (last || !ok) break;
+#pragma unroll
+            for (int h = 0; h < G; h++) al_prev[h] = al[h];
+            g++;
+            if (++i == w.cnt) {
+                i = 0;
+                kq++;
+                w.next();
+            }
         }
     } else {
         // ---- q in, results out --------------------------------------------------------------
+        if (start.done() && lane == 0) a.join[c] = make_int4(-1, 0, 0, 0);
         bool ok = true;
         int kq = 0;
         const int d0 = 8 * lane;
@@ -718,24 +720,29 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
             fence_proxy_async();
             mbar_arrive(&sm.q_full[qb]);
         };
-        Walk nx = start;  // the item whose q is staged next
-        if (!nx.done()) {
-            load_q(nx);
-            store_q(0);
-            nx.next();
-        }
-        for (Walk w = start; !w.done() && ok; w.next()) {
-            const size_t base = ((size_t)w.b * a.nq + w.h * G) * HD + d0;
-            if (!nx.done()) {
+        Walk nx = start, w = start;  // the item whose q is staged next; whose result is due
+        for (int kn = 0; ok;) {      // kn items staged: this one's and the next one's q, then its result
+            if (kn <= kq + 1 && !nx.done()) {
                 load_q(nx);
-                // the S MMAs of the item that used the buffer before are complete
-                if (kq + 1 >= QB)
-                    ok = bar_wait(&sm.q_empty[(kq + 1) % QB], ((kq + 1 - QB) / QB) & 1, &sm.abort,
-                                  status, VX_DEV_TIMEOUT_MMA);
+                if (kn >= QB)  // the S MMAs of the item that used the buffer before are complete
+                    ok = bar_wait(&sm.q_empty[kn % QB], ((kn - QB) / QB) & 1, &sm.abort, status,
+                                  VX_DEV_TIMEOUT_MMA);
                 ok = __all_sync(0xffffffffu, ok);
-                if (ok) store_q((kq + 1) % QB);
+                if (ok) store_q(kn % QB);
                 nx.next();
+                if (kn++ == 0 && lane == 0) {
+                    // an item that began in an earlier run is joined by the block of its second run
+                    int4 j = make_int4(-1, 0, 0, 0);
+                    if (w.v0 > 0) {
+                        const int c1 = owner(begin - w.v0), c2 = owner(begin - w.v0 + w.t.tiles - 1);
+                        if (c == c1 + 1) j = make_int4(w.b * nkv + w.h, c1, c2, 0);
+                    }
+                    a.join[c] = j;
+                }
+                continue;
             }
+            if (w.done()) break;
+            const size_t base = ((size_t)w.b * a.nq + w.h * G) * HD + d0;
             const bool whole = w.whole();
             float gv[G][8];
             if (whole && a.gate) {
@@ -766,8 +773,7 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
                     if (a.gate)
 #pragma unroll
                         for (int e = 0; e < 8; e++)
-                            o[h][e] *= TERMS == 2 ? __fdividef(1.0f, 1.0f + __expf(-gv[h][e]))
-                                                  : 1.0f / (1.0f + expf(-gv[h][e]));
+                            o[h][e] *= __fdividef(1.0f, 1.0f + __expf(-gv[h][e]));
                     if (a.out_bf16) st8_bf16(static_cast<uint16_t *>(a.out) + base + h * HD, o[h]);
                     else st8_f32(static_cast<float *>(a.out) + base + h * HD, o[h]);
                 }
@@ -779,6 +785,7 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
             // which runs hold the item, for the weight sums
             if (lane == 0 && a.scores && w.v0 == 0)
                 a.span[item] = make_int2(c, owner(end - w.left + w.t.tiles - 1));
+            w.next();
             kq++;
         }
     }
@@ -825,6 +832,14 @@ paged_join_k(const __grid_constant__ DecodeArgs a, int P, int G, int slot_blocks
         const int h = blk % G;
         if (j.x < 0) return;
         const int c1 = j.y, n = j.z - j.y + 1;
+        // one round trip: the gate, the (m, l) and the column's first values are requested together
+        const size_t i = ((size_t)(j.x / a.pool.nkv) * a.nq + (j.x % a.pool.nkv) * G + h) * HD + tid;
+        const float g = !a.gate ? 0.f : a.gate_bf16 ? act_ld<true>(a.gate, i) : act_ld<false>(a.gate, i);
+        constexpr int RU = 40;
+        float v[RU];
+#pragma unroll
+        for (int u = 0; u < RU; u++)
+            v[u] = u < n ? a.rec_o[(rec_of(c1, u) * G + h) * HD + tid] : 0.f;
         float m = -INFINITY;
         for (int r = tid; r < n; r += 256) m = fmaxf(m, a.rec_ml[rec_of(c1, r) * G + h].x);
         m = block_max(m);
@@ -834,24 +849,18 @@ paged_join_k(const __grid_constant__ DecodeArgs a, int P, int G, int slot_blocks
         }
         __syncthreads();
         float L = 0.f, O = 0.f;
-        for (int r0 = 0; r0 < n; r0 += 8) {
-            float v[8];
 #pragma unroll
-            for (int u = 0; u < 8; u++)
-                v[u] = r0 + u < n ? a.rec_o[(rec_of(c1, r0 + u) * G + h) * HD + tid] : 0.f;
-#pragma unroll
-            for (int u = 0; u < 8; u++) {
-                const float wr = r0 + u < n ? w_s[r0 + u] : 0.f;
-                L += wr;
-                O = fmaf(wr, v[u], O);
-            }
+        for (int u = 0; u < RU; u++) {
+            const float wr = u < n ? w_s[u] : 0.f;
+            L += wr;
+            O = fmaf(wr, v[u], O);
+        }
+        for (int r = RU; r < n; r++) {
+            L += w_s[r];
+            O = fmaf(w_s[r], a.rec_o[(rec_of(c1, r) * G + h) * HD + tid], O);
         }
         float o = O / L;
-        const size_t i = ((size_t)(j.x / a.pool.nkv) * a.nq + (j.x % a.pool.nkv) * G + h) * HD + tid;
-        if (a.gate) {
-            const float g = a.gate_bf16 ? act_ld<true>(a.gate, i) : act_ld<false>(a.gate, i);
-            o *= 1.0f / (1.0f + expf(-g));
-        }
+        if (a.gate) o *= 1.0f / (1.0f + expf(-g));
         if (a.out_bf16) act_st<true>(a.out, i, o);
         else act_st<false>(a.out, i, o);
         return;

@@ -166,9 +166,15 @@ def _need(t, name: str, numel: int, dtypes, optional: bool = False) -> None:
         raise Vx27Error(f"{name}: {t.numel()} elements, the call needs {numel}")
 
 
+_dtypes = None
+
+
 def _dt():
-    import torch
-    return torch.float32, torch.bfloat16, torch.int32, torch.float64, torch.uint8
+    global _dtypes
+    if _dtypes is None:
+        import torch
+        _dtypes = torch.float32, torch.bfloat16, torch.int32, torch.float64, torch.uint8
+    return _dtypes
 
 
 def _check_deltanet(S, conv_ring, qkv, a, b, A_log, dt_bias, conv_w, pos, o, B, nqk, nv, hd,
@@ -567,58 +573,80 @@ def gqa_prefill(q_in, k_in, v_in, gate, q_norm_w, k_norm_w, rope, k_cache, v_cac
 
 
 # ------------------------------------------------------------ paged KV cache
-def _pool(k_pages, v_pages, hd: int) -> tuple[int, int, int]:
-    """(pages, KV heads, page size) of a pool [n_pages][nkv][page_size][hd]."""
-    bf16 = _dt()[1]
-    for t, nm in ((k_pages, "k_pages"), (v_pages, "v_pages")):
-        if t.dim() != 4 or t.shape != k_pages.shape or t.shape[3] != hd:
-            raise Vx27Error(f"{nm}: shape {tuple(t.shape)}, expected [n_pages][nkv][page_size][{hd}]"
-                            f" for both planes")
-        _need(t, nm, 0, (bf16,))
-    return k_pages.shape[:3]
+# These calls are short, so each tensor is checked and turned into its address in one step.
+def _dev(t) -> int:
+    """The current device if t is on it, else -2."""
+    d = t.get_device()
+    return d if d >= 0 and d == _device() else -2
 
 
-def _shape(t, name: str, shape: tuple, dtypes) -> None:
-    """Checks a tensor argument's dtype and exact shape."""
+def _ptr(t, name: str, shape, dtypes, dev: int) -> int:
+    """Address of a contiguous tensor of this shape and one of these dtypes on device dev (-2:
+    the types and shapes are still checked, before _call refuses the device)."""
+    if t.dtype in dtypes and t.shape == shape and t.get_device() == dev and t.is_contiguous():
+        return t.data_ptr()
     _need(t, name, 0, dtypes)
-    if tuple(t.shape) != shape:
-        raise Vx27Error(f"{name}: shape {tuple(t.shape)}, expected {shape}")
+    if t.shape != shape:
+        raise Vx27Error(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
+    return 0 if dev < 0 else _t(t)
+
+
+def _scratch(t, dev: int) -> tuple:
+    """Address and bytes of a workspace."""
+    return _ptr(t, "workspace", t.shape, (t.dtype,), dev), t.nbytes
+
+
+def _call(fn: str, first, dev: int, stream, *args) -> None:
+    if dev < 0:
+        _t(first)  # raises: not on the current device
+    e = errbuf()
+    check(getattr(load(), fn)(*args, _stream(stream), e, 512), e)
+
+
+def _dims(t, name: str, n: int, what: str) -> tuple:
+    """Shape of a tensor with n dimensions."""
+    if t.dim() != n:
+        raise Vx27Error(f"{name}: shape {tuple(t.shape)}, expected {what}")
+    return t.shape
+
+
+def _pool(k_pages, v_pages, hd: int, dev: int) -> tuple:
+    """Addresses of the planes of a pool, its pages, KV heads and page size."""
+    shape = k_pages.shape
+    if len(shape) != 4 or shape[3] != hd:
+        raise Vx27Error(f"k_pages: shape {tuple(shape)}, expected [n_pages][nkv][page_size][{hd}]")
+    bf16 = _dt()[1:2]
+    return (_ptr(k_pages, "k_pages", shape, bf16, dev), _ptr(v_pages, "v_pages", shape, bf16, dev),
+            *shape[:3])
 
 
 def gqa_paged_append(q_in, k_in, v_in, q_norm_w, k_norm_w, rope, pos, slots, page_table, k_pages,
                      v_pages, q_out, seq=None, eps: float = 1e-6, norm_one_plus: bool = False,
                      stream=None) -> None:
     """QK norm + RoPE + K/V store of n tokens into the pages of their sequences
-    (vx27_gqa_paged_append). q_in [n, nq, hd], k_in, v_in [n, nkv, hd]; pos and slots [n]
-    int32 (a slot below 0 stores nothing), seq [n] int32 or None (token i is sequence i's);
-    page_table [n_seqs, max_pages] int32; q_out [n, nq, hd], fp32 for gqa_paged_decode or bf16
-    for gqa_paged_prefill."""
+    (vx27_gqa_paged_append). q_in [n, nq, hd], k_in, v_in [n, nkv, hd]; q_norm_w, k_norm_w [hd];
+    rope [positions, rope_dim] (rope_table); pos and slots [n] int32 (a slot below 0 stores
+    nothing), seq [n] int32 or None (token i is sequence i's); page_table [n_seqs, max_pages]
+    int32; q_out [n, nq, hd], fp32 for gqa_paged_decode or bf16 for gqa_paged_prefill."""
     n, nq, hd = q_in.shape
     f32, bf16, i32, _, _ = _dt()
-    n_pages, nkv, ps = _pool(k_pages, v_pages, hd)
-    _need(q_in, "q_in", 0, (f32, bf16))
-    for t, nm in ((k_in, "k_in"), (v_in, "v_in")):
-        _shape(t, nm, (n, nkv, hd), (q_in.dtype,))
-    _need(q_norm_w, "q_norm_w", hd, (f32,))
-    _need(k_norm_w, "k_norm_w", hd, (f32,))
-    if rope.dim() != 2:
-        raise Vx27Error(f"rope: shape {tuple(rope.shape)}, expected [positions][rope_dim]")
-    _need(rope, "rope", 0, (f32,))
-    for t, nm in ((pos, "pos"), (slots, "slots")) + (((seq, "seq"),) if seq is not None else ()):
-        _shape(t, nm, (n,), (i32,))
-    if page_table.dim() != 2:
-        raise Vx27Error(f"page_table: shape {tuple(page_table.shape)}, expected [n_seqs][max_pages]")
-    _need(page_table, "page_table", 0, (i32,))
-    _shape(q_out, "q_out", (n, nq, hd), (f32, bf16))
-    flags = (F_ACT_BF16 if _is_bf16(q_in) else 0) | (F_OUT_BF16 if _is_bf16(q_out) else 0) | \
+    dev = _dev(q_in)
+    rope_len, rope_dim = _dims(rope, "rope", 2, "[positions][rope_dim]")
+    n_seqs, max_pages = _dims(page_table, "page_table", 2, "[n_seqs][max_pages]")
+    kp, vp, n_pages, nkv, ps = _pool(k_pages, v_pages, hd, dev)
+    act, kv = (q_in.dtype,), (n, nkv, hd)
+    flags = (F_ACT_BF16 if q_in.dtype == bf16 else 0) | (F_OUT_BF16 if q_out.dtype == bf16 else 0) | \
         (F_NORM_1P if norm_one_plus else 0)
-    e = errbuf()
-    rc = load().vx27_gqa_paged_append(_t(q_in), _t(k_in), _t(v_in), _t(q_norm_w), _t(k_norm_w),
-                                      _t(rope), rope.shape[0], _t(pos), _t(slots), _t(seq),
-                                      _t(page_table), page_table.shape[0], page_table.shape[1],
-                                      _t(k_pages), _t(v_pages), n_pages, ps, _t(q_out), n, nq, nkv,
-                                      hd, rope.shape[1], eps, flags, _stream(stream), e, 512)
-    check(rc, e)
+    _call(
+        "vx27_gqa_paged_append", q_in, dev, stream,
+        _ptr(q_in, "q_in", (n, nq, hd), (f32, bf16), dev), _ptr(k_in, "k_in", kv, act, dev),
+        _ptr(v_in, "v_in", kv, act, dev), _ptr(q_norm_w, "q_norm_w", (hd,), (f32,), dev),
+        _ptr(k_norm_w, "k_norm_w", (hd,), (f32,), dev), _ptr(rope, "rope", rope.shape, (f32,), dev),
+        rope_len, _ptr(pos, "pos", (n,), (i32,), dev), _ptr(slots, "slots", (n,), (i32,), dev),
+        None if seq is None else _ptr(seq, "seq", (n,), (i32,), dev),
+        _ptr(page_table, "page_table", page_table.shape, (i32,), dev), n_seqs, max_pages, kp, vp,
+        n_pages, ps, _ptr(q_out, "q_out", (n, nq, hd), (f32, bf16), dev), n, nq, nkv, hd, rope_dim,
+        eps, flags)
 
 
 def gqa_paged_workspace_bytes(B: int, nq: int, nkv: int, hd: int, max_slots: int, window: int = 0,
@@ -636,29 +664,24 @@ def gqa_paged_decode(q, gate, k_pages, v_pages, page_table, lens, out, workspace
     gqa_paged_append), gate [B, nq, hd] or None, out [B, nq, hd]; page_table [B, max_pages],
     lens [B] int32. weight_sum fp32 [B, nkv, max_pages * page_size] or None: the weight each
     slot got is added to it."""
-    B, nq, hd = q.shape
+    B, nq, hd = shape = q.shape
     f32, bf16, i32, _, _ = _dt()
-    n_pages, nkv, ps = _pool(k_pages, v_pages, hd)
-    _need(q, "q", 0, (f32,))
-    if gate is not None:
-        _shape(gate, "gate", (B, nq, hd), (f32, bf16))
-    if page_table.dim() != 2 or page_table.shape[0] != B:
-        raise Vx27Error(f"page_table: shape {tuple(page_table.shape)}, expected [{B}][max_pages]")
-    _need(page_table, "page_table", 0, (i32,))
-    max_pages = page_table.shape[1]
-    _shape(lens, "lens", (B,), (i32,))
-    _shape(out, "out", (B, nq, hd), (f32, bf16))
-    if weight_sum is not None:
-        _shape(weight_sum, "weight_sum", (B, nkv, max_pages * ps), (f32,))
-    flags = (F_ACT_BF16 if gate is not None and _is_bf16(gate) else 0) | \
-        (F_OUT_BF16 if _is_bf16(out) else 0)
-    e = errbuf()
-    rc = load().vx27_gqa_paged_decode(_t(q), _t(gate), _t(k_pages), _t(v_pages), n_pages, ps,
-                                      _t(page_table), max_pages, _t(lens), window, sinks,
-                                      _t(weight_sum), _t(out), _t(workspace),
-                                      workspace.numel() * workspace.element_size(), B, nq, nkv, hd,
-                                      n_parts, flags, _stream(stream), e, 512)
-    check(rc, e)
+    dev = _dev(q)
+    kp, vp, n_pages, nkv, ps = _pool(k_pages, v_pages, hd, dev)
+    max_pages = _dims(page_table, "page_table", 2, f"[{B}][max_pages]")[1]
+    flags = (F_ACT_BF16 if gate is not None and gate.dtype == bf16 else 0) | \
+        (F_OUT_BF16 if out.dtype == bf16 else 0)
+    _call(
+        "vx27_gqa_paged_decode", q, dev, stream,
+        _ptr(q, "q", shape, (f32,), dev),
+        None if gate is None else _ptr(gate, "gate", shape, (f32, bf16), dev), kp, vp, n_pages, ps,
+        _ptr(page_table, "page_table", (B, max_pages), (i32,), dev), max_pages,
+        _ptr(lens, "lens", (B,), (i32,), dev), window, sinks,
+        None if weight_sum is None else
+        _ptr(weight_sum, "weight_sum", (B, nkv, max_pages * ps), (f32,), dev),
+        _ptr(out, "out", shape, (f32, bf16), dev), *_scratch(workspace, dev),
+        B, nq, nkv, hd,
+        n_parts, flags)
 
 
 def gqa_paged_prefill_workspace_bytes(nkv: int, hd: int) -> int:
@@ -670,23 +693,18 @@ def gqa_paged_prefill(q, gate, k_pages, v_pages, page_table, out, workspace, s0:
     """Causal attention of T tokens of one sequence in slots s0 .. s0 + T - 1, already
     appended (vx27_gqa_paged_prefill); window and sinks as for gqa_paged_decode. q, gate
     (or None), out [T, nq, hd] bf16; page_table [max_pages] int32."""
-    T, nq, hd = q.shape
+    T, nq, hd = shape = q.shape
     _, bf16, i32, _, _ = _dt()
-    n_pages, nkv, ps = _pool(k_pages, v_pages, hd)
-    _need(q, "q", 0, (bf16,))
-    if gate is not None:
-        _shape(gate, "gate", (T, nq, hd), (bf16,))
-    if page_table.dim() != 1:
-        raise Vx27Error(f"page_table: shape {tuple(page_table.shape)}, expected [max_pages]")
-    _need(page_table, "page_table", 0, (i32,))
-    _shape(out, "out", (T, nq, hd), (bf16,))
-    e = errbuf()
-    rc = load().vx27_gqa_paged_prefill(_t(q), _t(gate), _t(k_pages), _t(v_pages), n_pages, ps,
-                                       _t(page_table), page_table.shape[0], s0, window, sinks,
-                                       _t(out), _t(workspace),
-                                       workspace.numel() * workspace.element_size(), T, nq, nkv, hd,
-                                       F_ACT_BF16 | F_OUT_BF16, _stream(stream), e, 512)
-    check(rc, e)
+    dev = _dev(q)
+    kp, vp, n_pages, nkv, ps = _pool(k_pages, v_pages, hd, dev)
+    max_pages, = _dims(page_table, "page_table", 1, "[max_pages]")
+    _call(
+        "vx27_gqa_paged_prefill", q, dev, stream,
+        _ptr(q, "q", shape, (bf16,), dev),
+        None if gate is None else _ptr(gate, "gate", shape, (bf16,), dev), kp, vp, n_pages, ps,
+        _ptr(page_table, "page_table", (max_pages,), (i32,), dev), max_pages, s0, window, sinks,
+        _ptr(out, "out", shape, (bf16,), dev), *_scratch(workspace, dev), T, nq, nkv, hd,
+        F_ACT_BF16 | F_OUT_BF16)
 
 
 def kv_evict(k_pages, v_pages, page_table, lens, weight_sum, page_table_out, lens_out,
@@ -697,23 +715,19 @@ def kv_evict(k_pages, v_pages, page_table, lens, weight_sum, page_table_out, len
     order to the pages of page_table_out [B, max_pages_out]. kept [B, nkv, keep] int32 gets
     their old slots (-1 behind the last)."""
     f32, _, i32, _, _ = _dt()
-    n_pages, nkv, ps = _pool(k_pages, v_pages, 256)
-    if page_table.dim() != 2 or page_table_out.dim() != 2:
-        raise Vx27Error("page_table, page_table_out: expected [B][max_pages]")
-    (B, mp), mo = page_table.shape, page_table_out.shape[1]
-    _need(page_table, "page_table", 0, (i32,))
-    _shape(page_table_out, "page_table_out", (B, mo), (i32,))
-    _shape(lens, "lens", (B,), (i32,))
-    _shape(lens_out, "lens_out", (B,), (i32,))
-    _shape(weight_sum, "weight_sum", (B, nkv, mp * ps), (f32,))
-    _shape(weight_sum_out, "weight_sum_out", (B, nkv, mo * ps), (f32,))
-    _shape(kept, "kept", (B, nkv, keep), (i32,))
-    e = errbuf()
-    rc = load().vx27_kv_evict(_t(k_pages), _t(v_pages), n_pages, ps, _t(page_table), mp, _t(lens),
-                              _t(weight_sum), _t(page_table_out), mo, _t(lens_out),
-                              _t(weight_sum_out), _t(kept), keep, sinks, recent, B, nkv, 256,
-                              _stream(stream), e, 512)
-    check(rc, e)
+    dev = _dev(lens)
+    kp, vp, n_pages, nkv, ps = _pool(k_pages, v_pages, 256, dev)
+    B, mp = _dims(page_table, "page_table", 2, "[B][max_pages]")
+    mo = _dims(page_table_out, "page_table_out", 2, "[B][max_pages_out]")[1]
+    _call(
+        "vx27_kv_evict", lens, dev, stream,
+        kp, vp, n_pages, ps, _ptr(page_table, "page_table", (B, mp), (i32,), dev), mp,
+        _ptr(lens, "lens", (B,), (i32,), dev),
+        _ptr(weight_sum, "weight_sum", (B, nkv, mp * ps), (f32,), dev),
+        _ptr(page_table_out, "page_table_out", (B, mo), (i32,), dev), mo,
+        _ptr(lens_out, "lens_out", (B,), (i32,), dev),
+        _ptr(weight_sum_out, "weight_sum_out", (B, nkv, mo * ps), (f32,), dev),
+        _ptr(kept, "kept", (B, nkv, keep), (i32,), dev), keep, sinks, recent, B, nkv, 256)
 
 
 def fill_normal(t, seed: int, stream_id: int, mean: float = 0.0, std: float = 1.0,
