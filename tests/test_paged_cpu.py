@@ -41,7 +41,7 @@ def _prefill(**o):
 
 
 def _evict(**o):
-    a = dict(kp=P(16), vp=P(32), n_pages=8, ps=16, table=P(4), mp=4, lens=P(4), ws=P(4),
+    a = dict(kp=P(16), vp=P(32), n_pages=8, ps=16, table=P(4), mp=4, lens=P(4), ws=P(16),
              table2=P(8), mp2=2, lens2=P(8), ws2=P(8), kept=P(4), keep=20, sinks=4, recent=8, B=2,
              nkv=4, hd=HD)
     a.update(o)
@@ -77,7 +77,7 @@ WINDOW = [(dict(window=-1), "window=-1"), (dict(window=4, sinks=-1), "sinks=-1")
         (dict(sinks=-1), "keep=20"), (dict(sinks=0x7fffffff, recent=0x7fffffff), "keep=20"),
         (dict(mp2=1), "1 pages"), (dict(mp2=0), "0 pages"), (dict(ws=None), "null pointer"),
         (dict(table2=P(4)), "an output is an input"), (dict(lens2=P(4)), "an output is an input"),
-        (dict(ws2=P(4)), "an output is an input"), (dict(vp=P(16)), "an output is an input")]),
+        (dict(ws2=P(16)), "an output is an input"), (dict(ws=P(20)), "16-byte aligned"), (dict(vp=P(16)), "an output is an input")]),
 ])
 def test_c_refusals(vxlib, name, make, cases):
     import re

@@ -10,17 +10,16 @@ namespace {
 
 constexpr int HD = PG_HD;
 
-// 8 consecutive activations.
-template <bool BF16>
-__device__ __forceinline__ void ld8(float (&x)[8], const void *p, size_t i) {
-    if constexpr (BF16) ld8_bf16(x, static_cast<const uint16_t *>(p) + i);
-    else ld8_f32(x, static_cast<const float *>(p) + i);
-}
-
 // ---- append ---------------------------------------------------------------------------
-// One warp per (token, head) row, 8 consecutive dims per lane; y = x * rsqrt(mean x^2 + eps)
-// * w, then the rotation (x0, x1) -> (x0 c - x1 s, x0 s + x1 c) of dims (i, i + rope_dim/2),
-// whose partner is rope_dim/16 lanes away. The square sum is a tree of fp32 sums.
+// y = x * rsqrt(mean x^2 + eps) * w, then the rotation (x0, x1) -> (x0 c - x1 s, x0 s + x1 c)
+// of dims (i, i + rope_dim / 2). A warp takes `rows` heads of one token, so that the token's
+// position, slot, page and rope row are looked up once, four heads' loads in flight at a
+// time. Lane l < rope_dim / 8 holds dims 4 l .. and their partners rope_dim / 2 + 4 l .., the
+// others 8 l .., so a rotation needs no other lane; lanes without one rotate by (1, 0). The
+// square sum is a tree of fp32 sums.
+// Bound by the activations' bytes when there are many tokens: 4096 tokens of 24 + 4 heads take
+// MEASURE_APPEND (one head per warp at a time, everything looked up per head: 53 us); few tokens
+// by the chain slot -> page -> store.
 struct AppendArgs {
     const void *q_in, *k_in, *v_in;
     const float *qw, *kw, *rope;
@@ -28,83 +27,130 @@ struct AppendArgs {
     uint16_t *kp, *vp;
     void *q_out;
     PagePool pool;
-    int rope_len, rope_dim, n_seqs, max_pages, n, nq;
+    int rope_len, rope_dim, n_seqs, max_pages, n, nq, rows;
     float eps;
     int one_p, q_bf16;
 };
+
+// A lane's 8 values of a row: 4 from d0 and 4 from d1.
+template <bool BF16>
+struct Row8 {
+    uint2 a[2];
+    __device__ __forceinline__ void load(const void *p, size_t i, int d0, int d1) {
+        const uint16_t *r = static_cast<const uint16_t *>(p) + i;
+        a[0] = *reinterpret_cast<const uint2 *>(r + d0);
+        a[1] = *reinterpret_cast<const uint2 *>(r + d1);
+    }
+    __device__ __forceinline__ float get(int e) const {
+        const uint32_t w = (e & 2) ? a[e >> 2].y : a[e >> 2].x;
+        return (e & 1) ? __uint_as_float(w & 0xffff0000u) : __uint_as_float(w << 16);
+    }
+};
+template <>
+struct Row8<false> {
+    float4 a[2];
+    __device__ __forceinline__ void load(const void *p, size_t i, int d0, int d1) {
+        const float *r = static_cast<const float *>(p) + i;
+        a[0] = *reinterpret_cast<const float4 *>(r + d0);
+        a[1] = *reinterpret_cast<const float4 *>(r + d1);
+    }
+    __device__ __forceinline__ float get(int e) const {
+        const float4 &f = a[e >> 2];
+        return (e & 3) == 0 ? f.x : (e & 3) == 1 ? f.y : (e & 3) == 2 ? f.z : f.w;
+    }
+};
+__device__ __forceinline__ void st_row_bf16(uint16_t *p, int d0, int d1, const float (&y)[8]) {
+    *reinterpret_cast<uint2 *>(p + d0) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+    *reinterpret_cast<uint2 *>(p + d1) = make_uint2(pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
+}
 
 template <bool ACT_BF16>
 __global__ void __launch_bounds__(256)
 paged_append_k(const __grid_constant__ AppendArgs a, uint32_t *status) {
     grid_dep_wait();
     grid_dep_launch();
-    const int lane = threadIdx.x & 31, d0 = lane * 8;
-    const int nkv = a.pool.nkv, nh = a.nq + nkv;
-    const long long n_rows = (long long)a.n * nh;
-    const int half = a.rope_dim / 2;
-    const bool rot = d0 < a.rope_dim, lo = d0 < half;
-    const int i0 = lo ? d0 : d0 - half;
-    const int partner = (lo ? lane + half / 8 : lane - half / 8) & 31;
-    for (long long item = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; item < n_rows;
-         item += ((long long)gridDim.x * blockDim.x) >> 5) {
-        const int t = (int)(item / nh), head = (int)(item % nh);
-        const bool is_q = head < a.nq;
-        const int h = is_q ? head : head - a.nq;
-        const size_t row = (is_q ? (size_t)t * a.nq + h : (size_t)t * nkv + h) * HD + d0;
-        float x[8], v[8];
-        ld8<ACT_BF16>(x, is_q ? a.q_in : a.k_in, row);
-        const int p = a.pos[t];
-        const bool p_ok = p >= 0 && p < a.rope_len;
-        size_t dst = 0;
-        bool store = false;
-        if (!is_q) {
-            const int slot = a.slots[t], b = a.seq ? a.seq[t] : t;
-            if (slot >= 0) {
-                bool ok = b >= 0 && b < a.n_seqs && (slot >> a.pool.ps_log) < a.max_pages;
-                const int page =
-                    ok ? a.table[(size_t)b * a.max_pages + (slot >> a.pool.ps_log)] : -1;
-                ok = ok && a.pool.has(page);
-                if (!ok) dev_flag(status, VX_DEV_BAD_ARG);
-                store = ok;
-                if (ok) dst = a.pool.row(page, h, slot) * HD + d0;
+    const int lane = threadIdx.x & 31;
+    const int nkv = a.pool.nkv, nh = a.nq + nkv, parts = (nh + a.rows - 1) / a.rows;
+    const long long item = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+    if (item >= (long long)a.n * parts) return;
+    const int t = (int)(item / parts), h0 = (int)(item % parts) * a.rows, h1 = min(h0 + a.rows, nh);
+    const bool rot = lane < a.rope_dim / 8;
+    const int d0 = rot ? 4 * lane : 8 * lane, d1 = rot ? a.rope_dim / 2 + 4 * lane : 8 * lane + 4;
+    // the token: position, slot and page are looked up while the first rows come
+    const int p = a.pos[t], slot = a.slots[t], b = a.seq ? a.seq[t] : t;
+    float wq[8], wk[8], c[4], s[4];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const int d = (e < 4 ? d0 : d1) + (e & 3);
+        wq[e] = a.qw[d] + (a.one_p ? 1.0f : 0.0f);
+        wk[e] = a.kw[d] + (a.one_p ? 1.0f : 0.0f);
+    }
+    const bool p_ok = p >= 0 && p < a.rope_len;
+    if (a.rope_dim && !p_ok && lane == 0) dev_flag(status, VX_DEV_BAD_ARG);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const bool on = rot && p_ok;
+        const float *rr = a.rope + (size_t)p * a.rope_dim + d0 + e;
+        c[e] = on ? rr[0] : 1.0f;
+        s[e] = on ? rr[a.rope_dim / 2] : 0.0f;
+    }
+    int page = -1;
+    if (slot >= 0 && h1 > a.nq) {
+        const bool ok = b >= 0 && b < a.n_seqs && (slot >> a.pool.ps_log) < a.max_pages;
+        if (ok) page = a.table[(size_t)b * a.max_pages + (slot >> a.pool.ps_log)];
+        if (!a.pool.has(page)) {
+            page = -1;
+            if (lane == 0) dev_flag(status, VX_DEV_BAD_ARG);
+        }
+    }
+    for (int h = h0; h < h1; h += 4) {
+        Row8<ACT_BF16> x[4], v[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int i = h + u;
+            if (i >= h1) continue;
+            const size_t row = i < a.nq ? ((size_t)t * a.nq + i) * HD : ((size_t)t * nkv + i - a.nq) * HD;
+            x[u].load(i < a.nq ? a.q_in : a.k_in, row, d0, d1);
+            if (i >= a.nq && page >= 0) v[u].load(a.v_in, row, d0, d1);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int i = h + u;
+            if (i >= h1) continue;
+            const bool is_q = i < a.nq;
+            float y[8], ss = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                y[e] = x[u].get(e);
+                ss = fmaf(y[e], y[e], ss);
             }
-            ld8<ACT_BF16>(v, a.v_in, row);
-        }
-        float c[8], s[8];
-        if (rot && p_ok) {
-            const float *rr = a.rope + (size_t)p * a.rope_dim + i0;
-            ld8<false>(c, rr, 0);
-            ld8<false>(s, rr, half);
-        }
-        float ss = 0.f;
+            ss = warp_sum(ss);
+            const float r = rsqrtf(ss * (1.0f / HD) + a.eps);
 #pragma unroll
-        for (int e = 0; e < 8; e++) ss = fmaf(x[e], x[e], ss);
-        ss = warp_sum(ss);
-        const float r = __fdiv_rn(1.0f, __fsqrt_rn(ss * (1.0f / HD) + a.eps));
-        const float *wp = (is_q ? a.qw : a.kw) + d0;
-        float y[8], yp[8];
+            for (int e = 0; e < 8; e++) y[e] = y[e] * r * (is_q ? wq[e] : wk[e]);
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float w = __ldg(wp + e);
-            y[e] = x[e] * r * (a.one_p ? w + 1.0f : w);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; e++) yp[e] = __shfl_sync(0xffffffffu, y[e], partner);
-        if (rot) {
-            if (!p_ok) {
-                dev_flag(status, VX_DEV_BAD_ARG);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    y[e] = lo ? fmaf(y[e], c[e], -yp[e] * s[e]) : fmaf(yp[e], s[e], y[e] * c[e]);
+            for (int e = 0; e < 4; e++) {
+                const float x0 = y[e], x1 = y[e + 4];
+                y[e] = fmaf(x0, c[e], -x1 * s[e]);
+                y[e + 4] = fmaf(x1, c[e], x0 * s[e]);
             }
-        }
-        if (is_q) {
-            if (a.q_bf16) st8_bf16(static_cast<uint16_t *>(a.q_out) + row, y);
-            else st8_f32(static_cast<float *>(a.q_out) + row, y);
-        } else if (store) {
-            st8_bf16(a.kp + dst, y);
-            st8_bf16(a.vp + dst, v);
+            if (is_q) {
+                const size_t row = ((size_t)t * a.nq + i) * HD;
+                if (a.q_bf16) {
+                    st_row_bf16(static_cast<uint16_t *>(a.q_out) + row, d0, d1, y);
+                } else {
+                    float *o = static_cast<float *>(a.q_out) + row;
+                    *reinterpret_cast<float4 *>(o + d0) = make_float4(y[0], y[1], y[2], y[3]);
+                    *reinterpret_cast<float4 *>(o + d1) = make_float4(y[4], y[5], y[6], y[7]);
+                }
+            } else if (page >= 0) {
+                const size_t row = a.pool.row(page, i - a.nq, slot) * HD;
+                st_row_bf16(a.kp + row, d0, d1, y);
+                float z[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) z[e] = v[u].get(e);
+                st_row_bf16(a.vp + row, d0, d1, z);
+            }
         }
     }
 }
@@ -163,8 +209,16 @@ int vx27_gqa_paged_append(const void *q_in, const void *k_in, const void *v_in,
     a.eps = eps;
     a.one_p = (flags & VX27_F_NORM_1P) != 0;
     a.q_bf16 = (flags & VX27_F_OUT_BF16) != 0;
-    const long long rows = (long long)n * (nq + nkv);
-    const int grid = (int)std::min<long long>((rows + 7) / 8, (long long)num_sms() * 8);
+    // heads per warp: four (one round of loads) until the warps fill the SMs, then more, for
+    // fewer lookups; in equal parts
+    const int nh = nq + nkv;
+    const long long rounds = (long long)n * ((nh + 3) / 4), fill = (long long)num_sms() * 32;
+    const int rows = (int)std::min<long long>(nh, 4 * std::max<long long>(1, rounds / fill));
+    const int parts = (nh + rows - 1) / rows;
+    a.rows = ((nh + parts - 1) / parts + 3) / 4 * 4;
+    const long long warps = (long long)n * ((nh + a.rows - 1) / a.rows);
+    if (warps > (1LL << 33)) return fail(err, errlen, "%s: n=%d", fn, n);
+    const unsigned grid = (unsigned)((warps + 7) / 8);
     cudaStream_t st = (cudaStream_t)stream;
     if (flags & VX27_F_ACT_BF16)
         VX_CK(launch_pdl(paged_append_k<true>, dim3(grid), dim3(256), 0, st, a, dev_status()));

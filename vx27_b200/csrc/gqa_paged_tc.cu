@@ -800,7 +800,7 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
 // ---- join and weight sums ---------------------------------------------------------------
 // Blocks [0, B): zeros for a sequence without slots. Then (P - 1) G blocks: (c, h) merges head h of the item that run c continues, if c is
 // the second run of it: o = sum_r w_r o_r / sum_r w_r, w_r = l_r 2^(m_r - m). The other blocks
-// add the weights of 256 slots of an item: sum_h 2^(s_h - m_h) / l_h.
+// add the weights of 1024 slots of an item: sum_h 2^(s_h - m_h) / l_h.
 __global__ void __launch_bounds__(256)
 paged_join_k(const __grid_constant__ DecodeArgs a, int P, int G, int slot_blocks) {
     grid_dep_wait();
@@ -865,35 +865,55 @@ paged_join_k(const __grid_constant__ DecodeArgs a, int P, int G, int slot_blocks
         else act_st<false>(a.out, i, o);
         return;
     }
-    const int bi = blk - n_join, item = bi / slot_blocks;
-    const int b = item / a.pool.nkv, k = (bi % slot_blocks) * 256 + tid;
-    const SeqTiles t(seq_len(a, b), a.window, a.sinks);
-    if ((bi % slot_blocks) * 256 >= t.tiles * TILE) return;
-    const int2 span = a.span[item];
-    const int n = span.y - span.x + 1;
-    const int slot = t.first_slot(k / TILE) + k % TILE;
-    const bool valid = k < t.tiles * TILE && t.see.sees(slot);
-    const float *sc = a.scores + (size_t)item * G * a.score_stride + k;
-    float sum = 0.f;
-    for (int h = 0; h < G; h++) {
-        float m, L;
+    // 4 slots a thread; the scores are requested before the statistics, which warp h makes for
+    // head h
+    const int bi = blk - n_join, item = bi / slot_blocks, k0 = (bi % slot_blocks) * 1024 + 4 * tid;
+    const SeqTiles t(seq_len(a, item / a.pool.nkv), a.window, a.sinks);
+    if ((bi % slot_blocks) * 1024 >= t.tiles * TILE) return;
+    const float *sc = a.scores + (size_t)item * G * a.score_stride + k0;
+    float4 x[8];
+#pragma unroll
+    for (int h = 0; h < 8; h++)
+        x[h] = h < G && k0 < t.tiles * TILE
+                   ? *reinterpret_cast<const float4 *>(sc + (size_t)h * a.score_stride)
+                   : make_float4(0, 0, 0, 0);
+    __shared__ float2 ml_s[8];
+    if (warp < G) {
+        const int2 span = a.span[item];
+        const int n = span.y - span.x + 1;
+        float2 ml = make_float2(-INFINITY, 0.f);
         if (n == 1) {
-            const float2 ml = a.item_ml[(size_t)item * G + h];
-            m = ml.x;
-            L = ml.y;
+            ml = a.item_ml[(size_t)item * G + warp];
         } else {
-            m = -INFINITY;
-            for (int r = tid; r < n; r += 256) m = fmaxf(m, a.rec_ml[rec_of(span.x, r) * G + h].x);
-            m = block_max(m);
-            L = 0.f;
-            for (int r = 0; r < n; r++) {
-                const float2 ml = a.rec_ml[rec_of(span.x, r) * G + h];
-                L = fmaf(ml.y, exp2f(ml.x - m), L);
+            for (int r = lane; r < n; r += 32)
+                ml.x = fmaxf(ml.x, a.rec_ml[rec_of(span.x, r) * G + warp].x);
+            ml.x = warp_max(ml.x);
+            for (int r = lane; r < n; r += 32) {
+                const float2 e = a.rec_ml[rec_of(span.x, r) * G + warp];
+                ml.y = fmaf(e.y, exp2f(e.x - ml.x), ml.y);
             }
+            ml.y = warp_sum(ml.y);
         }
-        if (valid) sum += exp2f(sc[(size_t)h * a.score_stride] - m) / L;
+        if (lane == 0) ml_s[warp] = make_float2(ml.x, 1.0f / ml.y);
     }
-    if (valid) a.wsum[(size_t)item * (a.max_pages << a.pool.ps_log) + slot] += sum;
+    __syncthreads();
+    float4 sum = make_float4(0, 0, 0, 0);
+#pragma unroll
+    for (int h = 0; h < 8; h++) {
+        if (h >= G) break;
+        const float2 ml = ml_s[h];
+        sum.x = fmaf(exp2f(x[h].x - ml.x), ml.y, sum.x);
+        sum.y = fmaf(exp2f(x[h].y - ml.x), ml.y, sum.y);
+        sum.z = fmaf(exp2f(x[h].z - ml.x), ml.y, sum.z);
+        sum.w = fmaf(exp2f(x[h].w - ml.x), ml.y, sum.w);
+    }
+    if (k0 >= t.tiles * TILE) return;
+    const int slot = t.first_slot(k0 / TILE) + k0 % TILE;
+    float *ws = a.wsum + (size_t)item * ((size_t)a.max_pages << a.pool.ps_log) + slot;
+    if (t.see.sees(slot)) ws[0] += sum.x;
+    if (t.see.sees(slot + 1)) ws[1] += sum.y;
+    if (t.see.sees(slot + 2)) ws[2] += sum.z;
+    if (t.see.sees(slot + 3)) ws[3] += sum.w;
 }
 
 }  // namespace
@@ -946,7 +966,7 @@ int launch_paged_decode(const DecodeArgs &a, const void *k_pages, const void *v_
         make_tmap_bf16_2d(&mv16, v_pages, rows, HD, HD * 2, 64, 16, err, errlen))
         return -1;
     const int G = a.nq / a.pool.nkv;
-    const int slot_blocks = a.scores ? (int)((a.score_stride + 255) / 256) : 0;
+    const int slot_blocks = a.scores ? (int)((a.score_stride + 1023) / 1024) : 0;
     const long long blocks = a.B + (long long)(P - 1) * G + (long long)slot_blocks * a.B * a.pool.nkv;
     if (blocks > 0x7fffffffLL)
         return fail(err, errlen, "vx27_gqa_paged_decode: weight sums over %d sequences of %zu slots",
