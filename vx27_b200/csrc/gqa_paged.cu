@@ -12,14 +12,15 @@ constexpr int HD = PG_HD;
 
 // ---- append ---------------------------------------------------------------------------
 // y = x * rsqrt(mean x^2 + eps) * w, then the rotation (x0, x1) -> (x0 c - x1 s, x0 s + x1 c)
-// of dims (i, i + rope_dim / 2). A warp takes `rows` heads of one token, so that the token's
-// position, slot, page and rope row are looked up once, four heads' loads in flight at a
-// time. Lane l < rope_dim / 8 holds dims 4 l .. and their partners rope_dim / 2 + 4 l .., the
+// of dims (i, i + rope_dim / 2). A warp takes `rows` rows (q, k or v) of one token, so that its
+// position, slot, page and rope row are looked up once; the loads of four rows are in flight
+// while the four before them are worked on. Lane l < rope_dim / 8 holds dims 4 l .. and their partners rope_dim / 2 + 4 l .., the
 // others 8 l .., so a rotation needs no other lane; lanes without one rotate by (1, 0). The
 // square sum is a tree of fp32 sums.
 // Bound by the activations' bytes when there are many tokens: 4096 tokens of 24 + 4 heads take
-// MEASURE_APPEND (one head per warp at a time, everything looked up per head: 53 us); few tokens
-// by the chain slot -> page -> store.
+// 32 us, 4.2 TB/s (one head per warp at a time, everything looked up per head: 53 us); one
+// token takes 3.1 us, the chain slot -> page -> store.
+constexpr int APPEND_THREADS = 128;
 struct AppendArgs {
     const void *q_in, *k_in, *v_in;
     const float *qw, *kw, *rope;
@@ -65,12 +66,12 @@ __device__ __forceinline__ void st_row_bf16(uint16_t *p, int d0, int d1, const f
 }
 
 template <bool ACT_BF16>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(APPEND_THREADS, ACT_BF16 ? 6 : 4)
 paged_append_k(const __grid_constant__ AppendArgs a, uint32_t *status) {
     grid_dep_wait();
     grid_dep_launch();
     const int lane = threadIdx.x & 31;
-    const int nkv = a.pool.nkv, nh = a.nq + nkv, parts = (nh + a.rows - 1) / a.rows;
+    const int nkv = a.pool.nkv, nh = a.nq + 2 * nkv, parts = (nh + a.rows - 1) / a.rows;
     const long long item = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
     if (item >= (long long)a.n * parts) return;
     const int t = (int)(item / parts), h0 = (int)(item % parts) * a.rows, h1 = min(h0 + a.rows, nh);
@@ -79,21 +80,25 @@ paged_append_k(const __grid_constant__ AppendArgs a, uint32_t *status) {
     // the token: position, slot and page are looked up while the first rows come
     const int p = a.pos[t], slot = a.slots[t], b = a.seq ? a.seq[t] : t;
     float wq[8], wk[8], c[4], s[4];
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const int d = (e < 4 ? d0 : d1) + (e & 3);
-        wq[e] = a.qw[d] + (a.one_p ? 1.0f : 0.0f);
-        wk[e] = a.kw[d] + (a.one_p ? 1.0f : 0.0f);
-    }
+    auto weights = [&](float (&w)[8], const float *from) {
+        const float4 f = *reinterpret_cast<const float4 *>(from + d0);
+        const float4 g = *reinterpret_cast<const float4 *>(from + d1);
+        const float one = a.one_p ? 1.0f : 0.0f;
+        w[0] = f.x + one; w[1] = f.y + one; w[2] = f.z + one; w[3] = f.w + one;
+        w[4] = g.x + one; w[5] = g.y + one; w[6] = g.z + one; w[7] = g.w + one;
+    };
+    weights(wq, a.qw);
+    weights(wk, a.kw);
     const bool p_ok = p >= 0 && p < a.rope_len;
     if (a.rope_dim && !p_ok && lane == 0) dev_flag(status, VX_DEV_BAD_ARG);
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-        const bool on = rot && p_ok;
-        const float *rr = a.rope + (size_t)p * a.rope_dim + d0 + e;
-        c[e] = on ? rr[0] : 1.0f;
-        s[e] = on ? rr[a.rope_dim / 2] : 0.0f;
+    float4 cs = make_float4(1.f, 1.f, 1.f, 1.f), sn = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (rot && p_ok) {
+        const float *rr = a.rope + (size_t)p * a.rope_dim + d0;
+        cs = *reinterpret_cast<const float4 *>(rr);
+        sn = *reinterpret_cast<const float4 *>(rr + a.rope_dim / 2);
     }
+    c[0] = cs.x; c[1] = cs.y; c[2] = cs.z; c[3] = cs.w;
+    s[0] = sn.x; s[1] = sn.y; s[2] = sn.z; s[3] = sn.w;
     int page = -1;
     if (slot >= 0 && h1 > a.nq) {
         const bool ok = b >= 0 && b < a.n_seqs && (slot >> a.pool.ps_log) < a.max_pages;
@@ -103,29 +108,38 @@ paged_append_k(const __grid_constant__ AppendArgs a, uint32_t *status) {
             if (lane == 0) dev_flag(status, VX_DEV_BAD_ARG);
         }
     }
-    for (int h = h0; h < h1; h += 4) {
-        Row8<ACT_BF16> x[4], v[4];
+    auto request = [&](Row8<ACT_BF16> (&x)[4], int h) {
 #pragma unroll
         for (int u = 0; u < 4; u++) {
             const int i = h + u;
             if (i >= h1) continue;
-            const size_t row = i < a.nq ? ((size_t)t * a.nq + i) * HD : ((size_t)t * nkv + i - a.nq) * HD;
-            x[u].load(i < a.nq ? a.q_in : a.k_in, row, d0, d1);
-            if (i >= a.nq && page >= 0) v[u].load(a.v_in, row, d0, d1);
+            const int j = i < a.nq ? i : i < a.nq + nkv ? i - a.nq : i - a.nq - nkv;
+            x[u].load(i < a.nq ? a.q_in : i < a.nq + nkv ? a.k_in : a.v_in,
+                      ((size_t)t * (i < a.nq ? a.nq : nkv) + j) * HD, d0, d1);
         }
+    };
+    Row8<ACT_BF16> x[4], next[4];
+    request(next, h0);
+    for (int h = h0; h < h1; h += 4) {
+#pragma unroll
+        for (int u = 0; u < 4; u++) x[u] = next[u];
+        request(next, h + 4);
 #pragma unroll
         for (int u = 0; u < 4; u++) {
             const int i = h + u;
             if (i >= h1) continue;
-            const bool is_q = i < a.nq;
-            float y[8], ss = 0.f;
+            float y[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                y[e] = x[u].get(e);
-                ss = fmaf(y[e], y[e], ss);
+            for (int e = 0; e < 8; e++) y[e] = x[u].get(e);
+            if (i >= a.nq + nkv) {
+                if (page >= 0) st_row_bf16(a.vp + a.pool.row(page, i - a.nq - nkv, slot) * HD, d0, d1, y);
+                continue;
             }
-            ss = warp_sum(ss);
-            const float r = rsqrtf(ss * (1.0f / HD) + a.eps);
+            const bool is_q = i < a.nq;
+            float ss = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) ss = fmaf(y[e], y[e], ss);
+            const float r = rsqrtf(warp_sum(ss) * (1.0f / HD) + a.eps);
 #pragma unroll
             for (int e = 0; e < 8; e++) y[e] = y[e] * r * (is_q ? wq[e] : wk[e]);
 #pragma unroll
@@ -134,22 +148,14 @@ paged_append_k(const __grid_constant__ AppendArgs a, uint32_t *status) {
                 y[e] = fmaf(x0, c[e], -x1 * s[e]);
                 y[e + 4] = fmaf(x1, c[e], x0 * s[e]);
             }
-            if (is_q) {
-                const size_t row = ((size_t)t * a.nq + i) * HD;
-                if (a.q_bf16) {
-                    st_row_bf16(static_cast<uint16_t *>(a.q_out) + row, d0, d1, y);
-                } else {
-                    float *o = static_cast<float *>(a.q_out) + row;
-                    *reinterpret_cast<float4 *>(o + d0) = make_float4(y[0], y[1], y[2], y[3]);
-                    *reinterpret_cast<float4 *>(o + d1) = make_float4(y[4], y[5], y[6], y[7]);
-                }
-            } else if (page >= 0) {
-                const size_t row = a.pool.row(page, i - a.nq, slot) * HD;
-                st_row_bf16(a.kp + row, d0, d1, y);
-                float z[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) z[e] = v[u].get(e);
-                st_row_bf16(a.vp + row, d0, d1, z);
+            if (!is_q) {
+                if (page >= 0) st_row_bf16(a.kp + a.pool.row(page, i - a.nq, slot) * HD, d0, d1, y);
+            } else if (a.q_bf16) {
+                st_row_bf16(static_cast<uint16_t *>(a.q_out) + ((size_t)t * a.nq + i) * HD, d0, d1, y);
+            } else {
+                float *o = static_cast<float *>(a.q_out) + ((size_t)t * a.nq + i) * HD;
+                *reinterpret_cast<float4 *>(o + d0) = make_float4(y[0], y[1], y[2], y[3]);
+                *reinterpret_cast<float4 *>(o + d1) = make_float4(y[4], y[5], y[6], y[7]);
             }
         }
     }
@@ -183,8 +189,9 @@ int vx27_gqa_paged_append(const void *q_in, const void *k_in, const void *v_in,
         (rope_dim && (!rope_table || rope_table_len <= 0)))
         return fail(err, errlen, "%s: null pointer argument", fn);
     if (((uintptr_t)q_in | (uintptr_t)k_in | (uintptr_t)v_in | (uintptr_t)q_out |
-         (uintptr_t)rope_table) & 15)
-        return fail(err, errlen, "%s: activations, rope_table and q_out must be 16-byte aligned", fn);
+         (uintptr_t)q_norm_w | (uintptr_t)k_norm_w | (uintptr_t)rope_table) & 15)
+        return fail(err, errlen,
+                    "%s: activations, norm weights, rope_table and q_out must be 16-byte aligned", fn);
     AppendArgs a{};
     a.q_in = q_in;
     a.k_in = k_in;
@@ -211,19 +218,19 @@ int vx27_gqa_paged_append(const void *q_in, const void *k_in, const void *v_in,
     a.q_bf16 = (flags & VX27_F_OUT_BF16) != 0;
     // heads per warp: four (one round of loads) until the warps fill the SMs, then more, for
     // fewer lookups; in equal parts
-    const int nh = nq + nkv;
+    const int nh = nq + 2 * nkv;
     const long long rounds = (long long)n * ((nh + 3) / 4), fill = (long long)num_sms() * 32;
     const int rows = (int)std::min<long long>(nh, 4 * std::max<long long>(1, rounds / fill));
     const int parts = (nh + rows - 1) / rows;
     a.rows = ((nh + parts - 1) / parts + 3) / 4 * 4;
     const long long warps = (long long)n * ((nh + a.rows - 1) / a.rows);
     if (warps > (1LL << 33)) return fail(err, errlen, "%s: n=%d", fn, n);
-    const unsigned grid = (unsigned)((warps + 7) / 8);
+    const unsigned grid = (unsigned)((warps + APPEND_THREADS / 32 - 1) / (APPEND_THREADS / 32));
     cudaStream_t st = (cudaStream_t)stream;
     if (flags & VX27_F_ACT_BF16)
-        VX_CK(launch_pdl(paged_append_k<true>, dim3(grid), dim3(256), 0, st, a, dev_status()));
+        VX_CK(launch_pdl(paged_append_k<true>, dim3(grid), dim3(APPEND_THREADS), 0, st, a, dev_status()));
     else
-        VX_CK(launch_pdl(paged_append_k<false>, dim3(grid), dim3(256), 0, st, a, dev_status()));
+        VX_CK(launch_pdl(paged_append_k<false>, dim3(grid), dim3(APPEND_THREADS), 0, st, a, dev_status()));
     return 0;
 }
 
