@@ -436,6 +436,21 @@ def test_prompt_heads(cuda, nq, nkv):
         close(got, *prompt_ref(pool, q, gate, 90, window, sinks))
 
 
+@pytest.mark.parametrize("nq,nkv", [(24, 4), (5, 1), (2, 2)])
+@pytest.mark.parametrize("T,s0,window,sinks", [(1, 20000, 0, 0), (65, 7001, 0, 0), (300, 9000, 0, 0),
+                                               (200, 12000, 5000, 300), (1, 9000, 8999, 1),
+                                               (1500, 3000, 0, 0), (3000, 0, 2500, 4)])
+def test_prompt_few_rows_over_many_slots(cuda, nq, nkv, T, s0, window, sinks):
+    """Key tiles of a pair spread over several clusters, whose parts are joined; with a window
+    some rows see nothing of a part."""
+    g = gen(23)
+    pool = Pool(g, [s0 + T], nkv, 64)
+    q, gate = normal(g, T, nq, HD).to(BF), normal(g, T, nq, HD).to(BF)
+    for gt in (gate, None):
+        got = run_prompt(pool, q, gt, s0, window, sinks)
+        close(got, *prompt_ref(pool, q, gt, s0, window, sinks))
+
+
 def test_prompt_bad_page_is_reported(cuda):
     g = gen(14)
     pool = Pool(g, [300], 4, 16)
