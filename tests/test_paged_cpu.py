@@ -147,3 +147,71 @@ def test_wrapper_refusals():
             (dict(page_table_out=i(1, 2)), "page_table_out: shape")]:
         with pytest.raises(E, match=message):
             ev(**change)
+
+
+def cache(**o):
+    from vx27_b200.paged import PagedKV
+    return PagedKV(**(dict(layers=2, batch=3, n_pages=10, max_pages=4, page_size=16, nkv=1,
+                           device="cpu") | o))
+
+
+def held(c):
+    """Pages that the tables name, checked against the host's copy and the free list."""
+    pages = [p for row in c.table.tolist() for p in row if p >= 0]
+    assert c.table.tolist() == c._pages and c.lens.tolist() == c._lens
+    assert len(set(pages)) == len(pages) and sorted(pages + c._free) == list(range(len(c.k[0])))
+    return pages
+
+
+def test_paged_cache_hands_out_and_takes_back_pages():
+    c = cache()
+    assert c.extend({0: 17, 2: 16}) == {0: (0, 0), 2: (0, 0)}
+    assert len(held(c)) == 3 and c.lens.tolist() == [17, 0, 16] and c.free_pages == 7
+    assert c.extend({0: 15}) == {0: (17, 17)} and len(held(c)) == 3
+    assert c.extend({0: 1, 1: 1, 2: 33}) == {0: (32, 32), 1: (0, 0), 2: (16, 16)}
+    assert len(held(c)) == 8
+    with pytest.raises(ops.Vx27Error, match="3 pages needed, 2 free"):
+        c.extend({1: 60})
+    with pytest.raises(ops.Vx27Error, match="pass 4 pages of 16"):
+        c.extend({1: 1, 2: 16})
+    with pytest.raises(ops.Vx27Error, match="0 tokens"):
+        c.extend({1: 0})
+    assert len(held(c)) == 8 and c.lens.tolist() == [33, 1, 49]
+    c.release(2)
+    assert len(held(c)) == 4 and c.length(2) == c.position(2) == 0
+    c.extend({1: 60})
+    assert len(held(c)) == 7
+
+
+def test_paged_cache_frees_what_a_window_leaves():
+    c = cache(n_pages=6, max_pages=100, window=20, sinks=3)
+    total = 0
+    for n in (40, 1, 1, 30, 1, 500 - 73, 1):
+        if n > 60:  # more at once than the pages hold
+            with pytest.raises(ops.Vx27Error, match="free"):
+                c.extend({1: n})
+            continue
+        c.extend({1: n})
+        total += n
+        held(c)
+        have = [e for e, p in enumerate(c._pages[1]) if p >= 0]
+        # what the first of the new tokens saw, to the end, and the sinks
+        seen = {j // 16 for j in range(total) if j < 3 or j > total - n - 20}
+        assert set(have) == seen, (total, have, seen)
+    assert c.length(1) == c.position(1) == total
+
+
+def test_paged_cache_refusals():
+    with pytest.raises(ops.Vx27Error, match="one of the two"):
+        cache(window=4, weights=True)
+    c = cache()
+    with pytest.raises(ops.Vx27Error, match="weights=True"):
+        c.evict(4)
+    c = cache(weights=True)
+    assert c.evict(4) == ([], None)
+    c.extend({0: 64, 1: 60})
+    with pytest.raises(ops.Vx27Error, match="evict needs 4 free pages"):
+        c.evict(20)
+    with pytest.raises(ops.Vx27Error, match="keep=8"):
+        c.evict(8, sinks=4, recent=5)
+    held(c)

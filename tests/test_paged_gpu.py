@@ -698,3 +698,99 @@ def test_two_calls_at_once(cuda):
         ref, tol, _, _ = decode_ref(p, q, None, n, 0, 0, False, True)
         close(o, ref, tol)
     assert ops.device_status() == 0
+
+
+# ------------------------------------------------------------------ the layer over the cache
+def gqa_layer(seed, H=512, nq=12, nkv=2):
+    """A GQA layer with fp32 weights, as uploaded rows."""
+    from vx27_b200.layer import GQALayer, PackedLinear
+    g = gen(seed)
+
+    def lin(rows, cols):
+        w = normal(g, rows, cols) / cols ** 0.5
+        return PackedLinear(w.view(torch.uint8), ops.PMAT_F32, rows, cols)
+    return GQALayer(lin(nq * 2 * HD, H), lin(nkv * HD, H), lin(nkv * HD, H), lin(H, nq * HD),
+                    0.02 * normal(g, HD), 0.02 * normal(g, HD), ops.rope_table(512), nq, nkv)
+
+
+def test_layer_over_pages_matches_the_contiguous_cache(cuda):
+    """GQALayer.step_paged against GQALayer.step, token by token, an idle lane among them: the
+    same projections, so the outputs differ by the attention's and norms' rounding (both within
+    1e-5 of the formulas; 1e-4 of the largest value leaves room for the K rows that round to
+    the other bf16 neighbour, one in ~1000 by 2^-8 of its size)."""
+    from vx27_b200.paged import PagedKV
+    layer, B, cap, H = gqa_layer(30), 3, 64, 512
+    g = gen(31)
+    kc, vc = (torch.zeros(2, 2, cap, HD, device="cuda", dtype=BF) for _ in range(2))
+    ws = torch.empty(ops.gqa_workspace_bytes(2, 12, 2, HD, cap) // 4 + 1, device="cuda")
+    cache = PagedKV(1, B, 12, 4, 16, 2)
+    cw = cache.workspace(12)
+    for t in range(40):
+        x = normal(g, B, H)
+        at = cache.extend({0: 1, 2: 1})
+        assert at[0] == at[2] == (t, t)
+        pos = i32([t, 0, t])
+        got = layer.step_paged(x, cache, 0, pos, cw)
+        ref = layer.step(x[[0, 2]], kc, vc, i32([t, t]), ws)
+        assert float((got[[0, 2]] - ref).abs().max()) <= 1e-4 * float(ref.abs().max())
+        assert (got[1] == 0).all()
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("window,sinks,weights", [(0, 0, True), (50, 4, False)])
+def test_layer_prompt_then_steps(cuda, window, sinks, weights):
+    """A prompt through prompt_paged, in two parts, then tokens through step_paged, with pages
+    freed behind a window or the cache cut back by evict, against the layer's formulas in 64
+    bits over the rows that the cache then holds (bf16 results in prompts: 2^-7 of the largest
+    value; 1e-4 in steps, as above)."""
+    from vx27_b200.paged import PagedKV
+    layer, H, T, nkv, nq = gqa_layer(32), 512, 150, 2, 12
+    g = gen(33)
+    cache = PagedKV(1, 2, 40, 20, 16, nkv, window=window, sinks=sinks, weights=weights)
+    ws = cache.workspace(nq)
+    wd = [m.W.view(torch.float32).view(m.rows, m.cols).double() for m in (layer.q, layer.o)]
+
+    def want(x, n0):
+        """x [n, H] at slots n0 ..: the formulas, the cache's own K and V rows."""
+        qg = (x.double() @ wd[0].T).view(len(x), nq, 2, HD)
+        q = append_ref(qg[:, :, 0], layer.q_norm_w, True, layer.rope, torch.tensor(at_pos))
+        out = []
+        for i in range(len(x)):
+            page = cache.table[seq].long()
+            s = torch.tensor(seen(n0 + i + 1, window, sinks), device="cuda")
+            k = cache.k[0][page[s // 16], :, s % 16].double().transpose(0, 1)
+            v = cache.v[0][page[s // 16], :, s % 16].double().transpose(0, 1)
+            o = attend(q[i].view(nkv, -1, HD), k, v)[0].reshape(nq, HD)
+            out.append((o * torch.sigmoid(qg[i, :, 1])).flatten() @ wd[1].T)
+        return torch.stack(out)
+    seq, done = 1, 0
+    for n in (T - 33, 33):
+        x = normal(g, n, H)
+        slot, pos = cache.extend({seq: n})[seq]
+        assert (slot, pos) == (done, done)
+        got = layer.prompt_paged(x, cache, 0, seq, slot, pos, ws)
+        at_pos = list(range(pos, pos + n))
+        ref = want(x, slot)
+        assert float((got - ref).abs().max()) <= 2.0 ** -7 * float(ref.abs().max())
+        done += n
+    free = cache.free_pages
+    for t in range(40):
+        if weights and t == 20:
+            cut, kept = cache.evict(64, sinks=4, recent=16)
+            assert cut == [seq] and kept.shape == (1, 1, nkv, 64) and cache.length(seq) == 64
+            assert cache.free_pages == 36 and cache.position(seq) == T + 20
+        x = normal(g, 2, H)
+        slot, pos = cache.extend({seq: 1})[seq]
+        got = layer.step_paged(x, cache, 0, i32([0, pos]), ws)
+        at_pos = [pos]
+        ref = want(x[1:], slot)
+        assert float((got[1] - ref[0]).abs().max()) <= 1e-4 * float(ref.abs().max())
+        assert (got[0] == 0).all()
+    if window:
+        assert cache.free_pages > free  # the prompt's pages behind the window
+    if weights:  # each token hands out 1 per head, 6 heads a KV head; eviction drops some
+        total = cache.sums[0, seq].sum(-1)
+        assert ((total > 6 * 20 - 0.01) & (total < 6 * 40)).all()
+    cache.release(seq)
+    assert cache.free_pages == 40
+    assert ops.device_status() == 0

@@ -14,6 +14,8 @@ GQA layer (src/vx27_qfwd.c:156-214):
   q/k RMSNorm(1 + w), RoPE, BF16 KV append               (vx27_gqa_append, NORM_1P)
   softmax(q k^T / 16) v * sigmoid(gate)                                 (K2)
   out = W_o att                                                          (K5)
+  over a contiguous cache (step), or over pages (step_paged; prompt_paged for the tokens of
+  a prompt: vx27_gqa_paged_append, vx27_gqa_paged_decode, vx27_gqa_paged_prefill)
 
 The input x is the layer's normalised hidden state, fp32 [B, H]. The input projections
 of a layer read the same x, so they run as one K5 launch (``vx27_pmat_multi_dev``); each
@@ -113,3 +115,45 @@ class GQALayer:
         att = torch.empty(B, self.nq, self.hd, device=x.device)
         ops.gqa_decode_batch(qn, gate, k_cache, v_cache, pos, att, workspace, stream=stream)
         return self.o(att.view(B, self.nq * self.hd), stream=stream)
+
+    def _project(self, x: torch.Tensor, stream) -> tuple:
+        """q, gate, k, v of x [n, H], fp32 [n, heads, hd]."""
+        n = x.shape[0]
+        qg, k, v = project(x, self.q, self.k, self.v, stream=stream)
+        qg = qg.view(n, self.nq, 2, self.hd)
+        return (qg[:, :, 0].contiguous(), qg[:, :, 1].contiguous(), k.view(n, self.nkv, self.hd),
+                v.view(n, self.nkv, self.hd))
+
+    def step_paged(self, x: torch.Tensor, cache, layer: int, pos: torch.Tensor,
+                   workspace: torch.Tensor) -> torch.Tensor:
+        """One token of every sequence of a paged.PagedKV, whose extend() has made room for it:
+        x [B, H] fp32; pos [B] int32 its positions. Lanes that hold no slots are idle (their
+        rows attend to nothing and store nothing); all others must have been extended by one
+        token. With weights=True the layer's weight sums grow. Returns [B, H] fp32."""
+        q_in, gate, k, v = self._project(x, None)
+        q = torch.empty_like(q_in)
+        ops.gqa_paged_append(q_in, k, v, self.q_norm_w, self.k_norm_w, self.rope, pos,
+                             cache.lens - 1, cache.table, cache.k[layer], cache.v[layer], q,
+                             eps=self.eps, norm_one_plus=True)
+        att = torch.empty_like(q)
+        ops.gqa_paged_decode(q, gate, cache.k[layer], cache.v[layer], cache.table, cache.lens, att,
+                             workspace, window=cache.window, sinks=cache.sinks,
+                             weight_sum=None if cache.sums is None else cache.sums[layer])
+        return self.o(att.view(x.shape[0], self.nq * self.hd))
+
+    def prompt_paged(self, x: torch.Tensor, cache, layer: int, seq: int, slot: int, pos: int,
+                     workspace: torch.Tensor) -> torch.Tensor:
+        """T prompt tokens of one sequence of a paged.PagedKV, whose extend() has made room for
+        them at (slot, pos): x [T, H] fp32. The attention runs in bf16. Returns [T, H] fp32."""
+        T = x.shape[0]
+        q_in, gate, k, v = self._project(x, None)
+        at = torch.arange(T, dtype=torch.int32, device=x.device)
+        q = torch.empty(q_in.shape, dtype=torch.bfloat16, device=x.device)
+        ops.gqa_paged_append(q_in, k, v, self.q_norm_w, self.k_norm_w, self.rope, at + pos, at + slot,
+                             cache.table, cache.k[layer], cache.v[layer], q,
+                             seq=torch.full_like(at, seq), eps=self.eps, norm_one_plus=True)
+        att = torch.empty_like(q)
+        ops.gqa_paged_prefill(q, gate.to(torch.bfloat16), cache.k[layer], cache.v[layer],
+                              cache.table[seq], att, workspace, s0=slot, window=cache.window,
+                              sinks=cache.sinks)
+        return self.o(att.float().view(T, self.nq * self.hd))

@@ -1,0 +1,164 @@
+"""A paged BF16 KV cache for the full-attention layers: the pool of pages, the sequences' page
+tables and lengths, and what moves pages between them (include/vx27_paged.h). The reference
+keeps one contiguous fp32 cache per layer and sequence (src/vx27_qfwd.c:183-185).
+
+All layers of a model hold the same tokens, so one table serves them: page p is a page of
+every layer's planes. The tables live on the device; a host copy decides which page goes
+where, so nothing is read back. Per sequence the cache holds
+
+    lens   slots held (on the device too: vx27_gqa_paged_decode reads it)
+    pos    positions taken so far; equal to lens until an eviction cuts the slots back
+
+``layer.GQALayer.step_paged`` and ``prompt_paged`` run a layer over it.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import ops
+from ._lib import Vx27Error
+
+
+class PagedKV:
+    def __init__(self, layers: int, batch: int, n_pages: int, max_pages: int, page_size: int = 64,
+                 nkv: int = 4, hd: int = 256, window: int = 0, sinks: int = 0,
+                 weights: bool = False, device="cuda"):
+        """n_pages pages for batch sequences of at most max_pages pages each. window, sinks: what
+        every token attends to (0: everything); pages that fall out of sight are freed. weights:
+        the attention each slot gets is summed, for evict."""
+        if weights and window:
+            raise Vx27Error("PagedKV: eviction keeps slots by their weights, a window by their age: "
+                            "one of the two")
+        dev = torch.device(device)
+        kw = dict(device=dev)
+        self.page_size, self.max_pages, self.window, self.sinks = page_size, max_pages, window, sinks
+        self.k = torch.empty(layers, n_pages, nkv, page_size, hd, dtype=torch.bfloat16, **kw)
+        self.v = torch.empty_like(self.k)
+        self.table = torch.full((batch, max_pages), -1, dtype=torch.int32, **kw)
+        self.lens = torch.zeros(batch, dtype=torch.int32, **kw)
+        self.sums = torch.zeros(layers, batch, nkv, max_pages * page_size, **kw) if weights else None
+        self._free = list(range(n_pages - 1, -1, -1))
+        self._pages = [[-1] * max_pages for _ in range(batch)]
+        self._lens, self._pos = [0] * batch, [0] * batch
+
+    # ------------------------------------------------------------------ bookkeeping (host)
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def length(self, seq: int) -> int:
+        return self._lens[seq]
+
+    def position(self, seq: int) -> int:
+        return self._pos[seq]
+
+    def _need(self, seq: int, n: int) -> list[int]:
+        """Table entries that n more slots of the sequence need a page for."""
+        if n < 1:
+            raise Vx27Error(f"PagedKV: {n} tokens for sequence {seq}")
+        last = self._lens[seq] + n
+        if last > self.max_pages * self.page_size:
+            raise Vx27Error(f"PagedKV: sequence {seq} holds {self._lens[seq]} slots, {n} more pass "
+                            f"{self.max_pages} pages of {self.page_size}")
+        return [e for e in range(self._lens[seq] // self.page_size, -(-last // self.page_size))
+                if self._pages[seq][e] < 0]
+
+    def _upload(self, seqs) -> None:
+        for s in seqs:
+            self.table[s].copy_(torch.tensor(self._pages[s], dtype=torch.int32))
+
+    def _upload_lens(self) -> None:
+        self.lens.copy_(torch.tensor(self._lens, dtype=torch.int32))
+
+    def _out_of_sight(self, seq: int) -> list[int]:
+        """Entries that no later token attends to."""
+        if not self.window:
+            return []
+        ps, lo = self.page_size, self._lens[seq] + 1 - self.window
+        first = -(-self.sinks // ps)
+        return [e for e in range(first, max(lo, 0) // ps) if self._pages[seq][e] >= 0]
+
+    def extend(self, tokens: dict[int, int]) -> dict[int, tuple[int, int]]:
+        """Makes room for tokens[seq] more tokens of each sequence and counts them as held:
+        (first slot, first position) by sequence. Pages that earlier calls moved out of sight of
+        a window are freed first. On the device the lengths are those after these tokens."""
+        need = {s: self._need(s, n) for s, n in tokens.items()}
+        changed = set()
+        for s in tokens:
+            for e in self._out_of_sight(s):
+                self._free.append(self._pages[s][e])
+                self._pages[s][e] = -1
+                changed.add(s)
+        if sum(map(len, need.values())) > len(self._free):
+            self._upload(changed)
+            raise Vx27Error(f"PagedKV: {sum(map(len, need.values()))} pages needed, "
+                            f"{len(self._free)} free")
+        at = {}
+        for s, n in tokens.items():
+            for e in need[s]:
+                self._pages[s][e] = self._free.pop()
+                changed.add(s)
+            at[s] = self._lens[s], self._pos[s]
+            self._lens[s] += n
+            self._pos[s] += n
+        self._upload(changed)
+        self._upload_lens()
+        return at
+
+    def release(self, seq: int) -> None:
+        """The sequence is done: its pages are free, its lane is idle."""
+        self._free += [p for p in self._pages[seq] if p >= 0]
+        self._pages[seq] = [-1] * self.max_pages
+        self._lens[seq] = self._pos[seq] = 0
+        self._upload([seq])
+        self._upload_lens()
+        if self.sums is not None:
+            self.sums[:, seq] = 0
+
+    # --------------------------------------------------------------------------- device
+    def evict(self, keep: int, sinks: int = 0, recent: int = 0, seqs=None):
+        """Cuts the sequences that hold more than keep slots (all, or those of seqs) back to keep
+        of them in every layer and head: the first sinks, the last recent, and those with the
+        largest summed weights (vx27_kv_evict). They need ceil(keep / page_size) free pages each
+        meanwhile; their old pages are free afterwards. Returns the sequences cut and their kept
+        slots [layers][n][nkv][keep]."""
+        if self.sums is None:
+            raise Vx27Error("PagedKV: evict needs weights=True")
+        cut = [s for s in (range(len(self._lens)) if seqs is None else seqs) if self._lens[s] > keep]
+        if not cut:
+            return [], None
+        n = -(-keep // self.page_size)
+        if n * len(cut) > len(self._free):
+            raise Vx27Error(f"PagedKV: evict needs {n * len(cut)} free pages, {len(self._free)} are")
+        if not 0 <= sinks <= sinks + recent <= keep or keep < 1:
+            raise Vx27Error(f"PagedKV: keep={keep} with sinks={sinks} and recent={recent}")
+        layers, nkv, dev = len(self.k), self.k.shape[2], self.k.device
+        new = [[self._free.pop() for _ in range(n)] for _ in cut]
+        rows = torch.tensor(cut, device=dev)
+        dst = torch.tensor(new, dtype=torch.int32, device=dev)
+        table, lens = self.table[rows], self.lens[rows]
+        lens_out = torch.empty_like(lens)
+        kept = torch.empty(layers, len(cut), nkv, keep, dtype=torch.int32, device=dev)
+        out = torch.empty(len(cut), nkv, n * self.page_size, device=dev)
+        for i in range(layers):
+            sums = self.sums[i, rows]
+            ops.kv_evict(self.k[i], self.v[i], table, lens, sums, dst, lens_out, out, kept[i], keep,
+                         sinks=sinks, recent=recent)
+            self.sums[i, rows] = 0
+            self.sums[i, rows, :, :n * self.page_size] = out
+        for s, pages in zip(cut, new):
+            self._free += [p for p in self._pages[s] if p >= 0]
+            self._pages[s] = pages + [-1] * (self.max_pages - n)
+            self._lens[s] = keep
+        self._upload(cut)
+        self._upload_lens()
+        return cut, kept
+
+    def workspace(self, nq: int) -> torch.Tensor:
+        """Scratch for decode and prompt calls over this cache (one stream's at a time)."""
+        nkv, hd = self.k.shape[2], self.k.shape[4]
+        need = max(ops.gqa_paged_workspace_bytes(len(self._lens), nq, nkv, hd,
+                                                 self.max_pages * self.page_size, self.window,
+                                                 self.sinks, self.sums is not None),
+                   ops.gqa_paged_prefill_workspace_bytes(nkv, hd))
+        return torch.empty(need, dtype=torch.uint8, device=self.k.device)
