@@ -2,7 +2,7 @@
 // sinks slots, the last recent ones and the middle slots with the largest weight sums stay.
 //   evict_select_k   the kept slots in order (kept, weight_sum_out, lens_out): one CTA per
 //                    (KV head, sequence) finds the smallest kept sum by a radix select over
-//                    the order-preserving bits, 8 at a time, then compacts the slots above it
+//                    the order-preserving bits, 11 at a time, then compacts the slots above it
 //   evict_copy_k     the kept K and V rows to their new pages, one warp per row pair
 #include <math.h>
 #include <algorithm>
@@ -52,9 +52,11 @@ __device__ __forceinline__ int warp_scan(int x, int lane) {
     return x;
 }
 
-// Four slots a thread and round. A round trip to the sums' row (L1 after the first pass) and a
-// few barriers per pass are what it takes, not bytes: 4 passes and the compaction over 5001
-// slots take 7 us (29 us with one thread walking the bins and one slot a thread and round).
+// Four slots a thread and round; 11 bits of the threshold a pass, counted in shared memory.
+// Bytes do not bound it: three passes over a row that the L1 holds, the barriers between them
+// and the compaction's round per 4096 slots do. With the copy, one sequence cut from 5001 slots
+// to 2048 takes 15 us (8 bits a pass, four passes: 18), 64 sequences of up to 4163 cut to 1024
+// take 96 us (113); sums that are all alike, and so one bin, take as long.
 __global__ void __launch_bounds__(SEL_THREADS)
 evict_select_k(const __grid_constant__ EvictArgs a, uint32_t *status) {
     grid_dep_wait();
@@ -79,42 +81,46 @@ evict_select_k(const __grid_constant__ EvictArgs a, uint32_t *status) {
     const int lo = a.sinks, hi = n - a.recent;
     int want = a.keep - a.sinks - a.recent;  // of the hi - lo middle slots; fewer than all
     const bool any = want > 0;
-    __shared__ int hist[256], sums[32], s_want;
+    constexpr int BINS = 2048, PER = BINS / SEL_THREADS;
+    __shared__ int hist[BINS], sums[32], s_want;
     __shared__ uint32_t s_prefix;
     uint32_t prefix = 0;
-    for (int shift = 24; any && shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
+    for (int pass = 0; any && pass < 3; pass++) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;  // digits of 11, 11 and 10 bits
+        const int bins = pass == 2 ? 1024 : 2048;
+        const uint32_t above = pass == 0 ? 0 : 0xffffffffu << (pass == 1 ? 21 : 10);
+        for (int i = tid; i < BINS; i += SEL_THREADS) hist[i] = 0;
         __syncthreads();
         for (int j0 = 0; j0 < n; j0 += 4 * SEL_THREADS) {
             const int j = j0 + 4 * tid;
-            const float4 f = j < n ? *reinterpret_cast<const float4 *>(ws + j) : make_float4(0, 0, 0, 0);
+            if (j >= n) continue;
+            const float4 f = *reinterpret_cast<const float4 *>(ws + j);
             const float w[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const uint32_t k = sum_key(w[e]);
-                const bool in = j + e >= lo && j + e < hi &&
-                                (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8)));
-                // lanes with the same digit add once
-                const int digit = in ? (int)((k >> shift) & 255) : -1;
-                const uint32_t same = __match_any_sync(0xffffffffu, digit);
-                if (in && lane == __ffs(same) - 1) atomicAdd(&hist[digit], __popc(same));
+                if (j + e >= lo && j + e < hi && ((k ^ prefix) & above) == 0)
+                    atomicAdd(&hist[(k >> shift) & (bins - 1)], 1);
             }
         }
         __syncthreads();
-        // counts from the largest digit down: thread i has digit 255 - i
-        int count = 0, incl = 0;
-        if (tid < 256) {
-            count = hist[255 - tid];
-            incl = warp_scan(count, lane);
-            if (lane == 31) sums[warp] = incl;
-        }
+        // counts from the largest digit down: thread i has digits BINS - 1 - PER i - (0 .. PER - 1)
+        int count[PER], mine = 0;
+#pragma unroll
+        for (int u = 0; u < PER; u++) mine += count[u] = hist[BINS - 1 - PER * tid - u];
+        int incl = warp_scan(mine, lane);
+        if (lane == 31) sums[warp] = incl;
         __syncthreads();
-        if (tid < 256) {
-            for (int w = 0; w < warp; w++) incl += sums[w];
-            if (incl >= want && incl - count < want) {  // one thread: the threshold's digit
-                s_want = want - (incl - count);
-                s_prefix = prefix | ((uint32_t)(255 - tid) << shift);
+        const int part = warp_scan(sums[lane], lane);
+        incl += warp ? __shfl_sync(0xffffffffu, part, warp - 1) : 0;
+        int upto = incl - mine;
+#pragma unroll
+        for (int u = 0; u < PER; u++) {
+            if (upto < want && upto + count[u] >= want) {  // one digit in all: the threshold's
+                s_want = want - upto;
+                s_prefix = prefix | ((uint32_t)(BINS - 1 - PER * tid - u) << shift);
             }
+            upto += count[u];
         }
         __syncthreads();
         want = s_want;
