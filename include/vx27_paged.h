@@ -8,7 +8,8 @@
  * device: slot s of sequence b is row s % page_size of every KV head of page
  * page_table[b][s / page_size]. A sequence's slots are numbered in the order in which its
  * tokens came. page_size is 16, 32, 64, 128 or 256, hd is 256, nq / nkv is 1 to 8; caches,
- * activations and outputs are 16-byte aligned and contiguous.
+ * activations, norm weights, weight sums, outputs and workspaces are 16-byte aligned and
+ * contiguous. A table holds at most 2^31 - 256 slots per sequence.
  *
  * A window keeps the last `window` slots in sight and the first `sinks` ones: with n slots
  * up to and with its own, a token attends to slot j when j >= n - window or j < sinks. window
@@ -62,10 +63,12 @@ int vx27_gqa_paged_append(const void *q_in, const void *k_in, const void *v_in,
  *   weight_sum fp32 [B][nkv][max_pages * page_size] or NULL: to the entry of each slot attended
  *   to, the softmax weights that the heads of its group gave it are added (vx27_kv_evict)
  *   workspace: vx27_gqa_paged_workspace_size(...) bytes, 16-byte aligned
- * The slots are split over the SMs, n_parts ways (0: the library's choice), and the parts
- * joined. With fp32 out or weight_sum, q and the softmax's weights enter the tensor cores as
- * three bf16 terms (24 bits), else as two (16 bits). The result does not depend on the other
- * sequences of the batch except through the automatic split count.
+ * The slots that the batch attends to are counted in tiles of 128 and cut into n_parts equal
+ * runs (0: one per SM; at most 1024), which are joined where a cut goes through a sequence. So the
+ * lengths of the other sequences move the cuts, and with them the last bits of a result; the
+ * same call always gives the same bits. With fp32 out or weight_sum, q and the softmax's
+ * weights enter the tensor cores as three bf16 terms (24 bits), else as two (16 bits).
+ * Batches of over 2^31 tiles are refused.
  */
 size_t vx27_gqa_paged_workspace_size(int B, int nq, int nkv, int hd, int max_slots, int window,
                                      int sinks, int weights, int n_parts);
@@ -82,7 +85,7 @@ int vx27_gqa_paged_decode(const float *q, const void *gate, const void *k_pages,
  *   q, gate, out [T][nq][hd] bf16 (gate may be NULL; the flags are VX27_F_ACT_BF16 |
  *   VX27_F_OUT_BF16, other types are refused: the softmax's weights enter the tensor cores
  *   as bf16); page_table [max_pages], the sequence's row
- *   workspace: vx27_gqa_paged_prefill_workspace_size(nkv, hd) bytes, 16-byte aligned
+ *   workspace: vx27_gqa_paged_prefill_workspace_size(nkv, hd) bytes (51 MB, whatever T)
  * K and V of the slots up to s0 + T - 1 in the pages that are attended to have to be
  * finite: a NaN or infinite V value reaches every token of its block of 128, masked or not.
  */
@@ -102,6 +105,8 @@ int vx27_gqa_paged_prefill(const void *q, const void *gate, const void *k_pages,
  *   lens, lens_out [B]; weight_sum [B][nkv][max_pages * page_size], weight_sum_out
  *   [B][nkv][max_pages_out * page_size] (zero behind the kept slots)
  *   kept int32 [B][nkv][keep]: the old slot of each new one, -1 behind the last
+ * Per head the kept slots differ, so afterwards a new slot's row is another token's in every
+ * head; rows of the new pages behind lens_out are left as they were.
  * sinks + recent <= keep <= max_pages_out * page_size. No page of page_table_out may be a page
  * of page_table or occur twice, and no output may be an input: a call whose output
  * pointers equal its input pointers is refused.

@@ -158,7 +158,9 @@ def cache(**o):
 def held(c):
     """Pages that the tables name, checked against the host's copy and the free list."""
     pages = [p for row in c.table.tolist() for p in row if p >= 0]
-    assert c.table.tolist() == c._pages and c.lens.tolist() == c._lens
+    assert c.table.tolist() == c._pages
+    assert c.lens.tolist() == c._lens and c.pos.tolist() == c._pos
+    assert all(a in (0, b) for a, b in zip(c.step.tolist(), c._lens))
     assert len(set(pages)) == len(pages) and sorted(pages + c._free) == list(range(len(c.k[0])))
     return pages
 
@@ -169,7 +171,7 @@ def test_paged_cache_hands_out_and_takes_back_pages():
     assert len(held(c)) == 3 and c.lens.tolist() == [17, 0, 16] and c.free_pages == 7
     assert c.extend({0: 15}) == {0: (17, 17)} and len(held(c)) == 3
     assert c.extend({0: 1, 1: 1, 2: 33}) == {0: (32, 32), 1: (0, 0), 2: (16, 16)}
-    assert len(held(c)) == 8
+    assert len(held(c)) == 8 and c.step.tolist() == [33, 1, 0]
     with pytest.raises(ops.Vx27Error, match="3 pages needed, 2 free"):
         c.extend({1: 60})
     with pytest.raises(ops.Vx27Error, match="pass 4 pages of 16"):
@@ -177,6 +179,11 @@ def test_paged_cache_hands_out_and_takes_back_pages():
     with pytest.raises(ops.Vx27Error, match="0 tokens"):
         c.extend({1: 0})
     assert len(held(c)) == 8 and c.lens.tolist() == [33, 1, 49]
+    for seqs in ({3: 1}, {-1: 1}):
+        with pytest.raises(ops.Vx27Error, match="sequences"):
+            c.extend(seqs)
+    with pytest.raises(ops.Vx27Error, match="sequences"):
+        c.release(-1)
     c.release(2)
     assert len(held(c)) == 4 and c.length(2) == c.position(2) == 0
     c.extend({1: 60})
@@ -204,6 +211,9 @@ def test_paged_cache_frees_what_a_window_leaves():
 def test_paged_cache_refusals():
     with pytest.raises(ops.Vx27Error, match="one of the two"):
         cache(window=4, weights=True)
+    for window, sinks in ((-1, 0), (4, -1), (0, 2)):
+        with pytest.raises(ops.Vx27Error, match="window="):
+            cache(window=window, sinks=sinks)
     c = cache()
     with pytest.raises(ops.Vx27Error, match="weights=True"):
         c.evict(4)
@@ -214,4 +224,7 @@ def test_paged_cache_refusals():
         c.evict(20)
     with pytest.raises(ops.Vx27Error, match="keep=8"):
         c.evict(8, sinks=4, recent=5)
+    for bad in ([1, 1], [-1], [3]):
+        with pytest.raises(ops.Vx27Error, match="sequences"):
+            c.evict(20, seqs=bad)
     held(c)

@@ -729,8 +729,7 @@ def test_layer_over_pages_matches_the_contiguous_cache(cuda):
         x = normal(g, B, H)
         at = cache.extend({0: 1, 2: 1})
         assert at[0] == at[2] == (t, t)
-        pos = i32([t, 0, t])
-        got = layer.step_paged(x, cache, 0, pos, cw)
+        got = layer.step_paged(x, cache, 0, cw)
         ref = layer.step(x[[0, 2]], kc, vc, i32([t, t]), ws)
         assert float((got[[0, 2]] - ref).abs().max()) <= 1e-4 * float(ref.abs().max())
         assert (got[1] == 0).all()
@@ -781,7 +780,7 @@ def test_layer_prompt_then_steps(cuda, window, sinks, weights):
             assert cache.free_pages == 36 and cache.position(seq) == T + 20
         x = normal(g, 2, H)
         slot, pos = cache.extend({seq: 1})[seq]
-        got = layer.step_paged(x, cache, 0, i32([0, pos]), ws)
+        got = layer.step_paged(x, cache, 0, ws)
         at_pos = [pos]
         ref = want(x[1:], slot)
         assert float((got[1] - ref[0]).abs().max()) <= 1e-4 * float(ref.abs().max())
@@ -793,4 +792,38 @@ def test_layer_prompt_then_steps(cuda, window, sinks, weights):
         assert ((total > 6 * 20 - 0.01) & (total < 6 * 40)).all()
     cache.release(seq)
     assert cache.free_pages == 40
+    assert ops.device_status() == 0
+
+
+def test_layer_step_replays_and_leaves_idle_lanes(cuda):
+    """A captured step_paged replayed after each extend gives the eager results bit for bit; a
+    sequence that an extend leaves out keeps its rows and sums."""
+    from vx27_b200.paged import PagedKV
+    layer, B, H = gqa_layer(34), 3, 512
+    g = gen(35)
+    caches = [PagedKV(1, B, 12, 4, 16, 2, weights=True) for _ in range(2)]
+    ws = [c.workspace(12) for c in caches]
+    prompt, x = normal(g, 30, H), torch.empty(B, H, device="cuda")
+    for c, w in zip(caches, ws):
+        c.k.zero_()
+        c.v.zero_()
+        layer.prompt_paged(prompt, c, 0, 1, *c.extend({1: 30})[1], w)
+    layer.step_paged(x.zero_(), caches[1], 0, ws[1])  # all lanes idle
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer.step_paged(x, caches[1], 0, ws[1])
+    for t in range(20):
+        tokens = {0: 1} if t % 3 == 0 else {1: 1} if t % 3 == 1 else {0: 1, 1: 1, 2: 1}
+        x.copy_(normal(g, B, H))
+        rows = {s: caches[1].sums[0, s].clone() for s in range(B) if s not in tokens}
+        for c in caches:
+            c.extend(tokens)
+        ref = layer.step_paged(x, caches[0], 0, ws[0])
+        graph.replay()
+        assert torch.equal(out, ref)
+        for s, before in rows.items():
+            assert (out[s] == 0).all() and torch.equal(caches[1].sums[0, s], before)
+    for name in ("k", "v", "sums", "table", "lens", "pos", "step"):
+        assert torch.equal(getattr(caches[0], name), getattr(caches[1], name)), name
     assert ops.device_status() == 0

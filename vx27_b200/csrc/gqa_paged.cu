@@ -14,9 +14,9 @@ constexpr int HD = PG_HD;
 // y = x * rsqrt(mean x^2 + eps) * w, then the rotation (x0, x1) -> (x0 c - x1 s, x0 s + x1 c)
 // of dims (i, i + rope_dim / 2). A warp takes `rows` rows (q, k or v) of one token, so that its
 // position, slot, page and rope row are looked up once; the loads of four rows are in flight
-// while the four before them are worked on. Lane l < rope_dim / 8 holds dims 4 l .. and their partners rope_dim / 2 + 4 l .., the
-// others 8 l .., so a rotation needs no other lane; lanes without one rotate by (1, 0). The
-// square sum is a tree of fp32 sums.
+// while the four before them are worked on. Lane l < rope_dim / 8 holds dims 4 l .. and their
+// partners rope_dim / 2 + 4 l .., the others 8 l .., so a rotation needs no other lane; lanes
+// without one rotate by (1, 0). The square sum is a tree of fp32 sums.
 // Bound by the activations' bytes when there are many tokens: 4096 tokens of 24 + 4 heads take
 // 32 us, 4.2 TB/s (one head per warp at a time, everything looked up per head: 53 us); one
 // token takes 3.1 us, the chain slot -> page -> store.

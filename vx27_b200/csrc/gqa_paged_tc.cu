@@ -16,15 +16,19 @@
 // x = hi + mid (+ lo), whose products with the bf16 cache are exact in fp32. Two terms carry
 // 16 bits (bf16 output), three 24 (fp32 output, weight sums).
 //
-// What bounds it: the cache bytes, 128 KB per tile through a ring of 12 chunks of 16 KB (128
-// slots x 64 dims) per SM, each tile's K and then its V by one warp. (Rings of their own for K
-// and V, by two warps, read memory in a worse order: 0.75 of its bandwidth instead of 0.84 over
-// 128 sequences of 2048 slots, whatever the split of the 12 slots.) A page is a box of its own: boxes of min(page_size, 128) rows
-// where all of them are seen, else boxes of the 16-row groups with a seen slot. The O MMAs
-// take 16 slots each and leave the other groups out; unseen rows of a copied group are zeroed.
+// What bounds it: the cache bytes, 128 KB per tile through two rings of 6 chunks of 16 KB (128
+// slots x 64 dims) per SM, one for K and one for V, each with a copying and a multiplying warp
+// of its own. 128 sequences of 2048 slots (1.07 GB) take 179-183 us, 0.89-0.915 of the copy
+// rate (0.84 with one ring, one copying and one multiplying warp, where a wait for K holds up
+// V). A small batch is bound by its chain instead: start and scan of the lengths 1.5 us,
+// first data 5, last result 2, join 3.5.
+// A page is a box of its own: boxes of min(page_size, 128) rows where all of them are seen,
+// else boxes of the 16-row groups with a seen slot. The O MMAs take 16 slots each and leave
+// the other groups out; unseen rows of a copied group are zeroed.
 //
-// Warps: 0 copies (lane i: rows 16 i .. of the tile), 1 issues the MMAs, 2-5 softmax and
-// accumulation, 6 q, gate and results. Waits are bounded (2 s).
+// Warps: 0 copies K and 7 copies V (lane i: rows 16 i .. of the tile; page ids come a tile
+// ahead), 1 issues the S MMAs and 8 the O MMAs, 2-5 softmax and accumulation, 6 q, gate and
+// results. Waits are bounded (2 s).
 #include <math.h>
 #include <algorithm>
 #include "common.cuh"

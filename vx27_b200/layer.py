@@ -124,19 +124,20 @@ class GQALayer:
         return (qg[:, :, 0].contiguous(), qg[:, :, 1].contiguous(), k.view(n, self.nkv, self.hd),
                 v.view(n, self.nkv, self.hd))
 
-    def step_paged(self, x: torch.Tensor, cache, layer: int, pos: torch.Tensor,
+    def step_paged(self, x: torch.Tensor, cache, layer: int,
                    workspace: torch.Tensor) -> torch.Tensor:
-        """One token of every sequence of a paged.PagedKV, whose extend() has made room for it:
-        x [B, H] fp32; pos [B] int32 its positions. Lanes that hold no slots are idle (their
-        rows attend to nothing and store nothing); all others must have been extended by one
-        token. With weights=True the layer's weight sums grow. Returns [B, H] fp32."""
+        """One token of each sequence of a paged.PagedKV that its last extend() gave one to: x
+        [B, H] fp32. The other lanes are idle: they store nothing and their rows come from a
+        zero attention output. With weights=True the layer's weight sums grow. Returns [B, H]
+        fp32."""
         q_in, gate, k, v = self._project(x, None)
         q = torch.empty_like(q_in)
-        ops.gqa_paged_append(q_in, k, v, self.q_norm_w, self.k_norm_w, self.rope, pos,
-                             cache.lens - 1, cache.table, cache.k[layer], cache.v[layer], q,
+        idle = cache.step == 0
+        ops.gqa_paged_append(q_in, k, v, self.q_norm_w, self.k_norm_w, self.rope,
+                             (cache.pos - 1).masked_fill_(idle, 0), cache.step - 1, cache.table, cache.k[layer], cache.v[layer], q,
                              eps=self.eps, norm_one_plus=True)
         att = torch.empty_like(q)
-        ops.gqa_paged_decode(q, gate, cache.k[layer], cache.v[layer], cache.table, cache.lens, att,
+        ops.gqa_paged_decode(q, gate, cache.k[layer], cache.v[layer], cache.table, cache.step, att,
                              workspace, window=cache.window, sinks=cache.sinks,
                              weight_sum=None if cache.sums is None else cache.sums[layer])
         return self.o(att.view(x.shape[0], self.nq * self.hd))

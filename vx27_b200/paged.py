@@ -4,12 +4,20 @@ keeps one contiguous fp32 cache per layer and sequence (src/vx27_qfwd.c:183-185)
 
 All layers of a model hold the same tokens, so one table serves them: page p is a page of
 every layer's planes. The tables live on the device; a host copy decides which page goes
-where, so nothing is read back. Per sequence the cache holds
+where, so nothing is read back. Per sequence the device holds (int32)
 
-    lens   slots held (on the device too: vx27_gqa_paged_decode reads it)
-    pos    positions taken so far; equal to lens until an eviction cuts the slots back
+    lens   slots held
+    pos    positions taken; equal to lens until an eviction cuts the slots back
+    step   lens, if the last extend() gave the sequence one token, else 0 (an idle lane)
 
-``layer.GQALayer.step_paged`` and ``prompt_paged`` run a layer over it.
+``layer.GQALayer.step_paged`` and ``prompt_paged`` run a layer over it. A round of a server:
+
+    at = cache.extend({0: 1, 1: 1, 5: 300})       # two running sequences, a new prompt
+    for each layer i: step_paged(x, cache, i, ws), prompt_paged(xp, cache, i, 5, *at[5], ws)
+
+The tensors keep their addresses, so a captured step_paged may be replayed after each
+extend(); extend, release and evict copy from the host and stay outside the capture. All
+calls on one cache belong on one stream.
 """
 from __future__ import annotations
 
@@ -26,6 +34,8 @@ class PagedKV:
         """n_pages pages for batch sequences of at most max_pages pages each. window, sinks: what
         every token attends to (0: everything); pages that fall out of sight are freed. weights:
         the attention each slot gets is summed, for evict."""
+        if window < 0 or sinks < 0 or (sinks and not window):
+            raise Vx27Error(f"PagedKV: window={window} with sinks={sinks}")
         if weights and window:
             raise Vx27Error("PagedKV: eviction keeps slots by their weights, a window by their age: "
                             "one of the two")
@@ -35,7 +45,8 @@ class PagedKV:
         self.k = torch.empty(layers, n_pages, nkv, page_size, hd, dtype=torch.bfloat16, **kw)
         self.v = torch.empty_like(self.k)
         self.table = torch.full((batch, max_pages), -1, dtype=torch.int32, **kw)
-        self.lens = torch.zeros(batch, dtype=torch.int32, **kw)
+        self._state = torch.zeros(3, batch, dtype=torch.int32, **kw)
+        self.lens, self.pos, self.step = self._state
         self.sums = torch.zeros(layers, batch, nkv, max_pages * page_size, **kw) if weights else None
         self._free = list(range(n_pages - 1, -1, -1))
         self._pages = [[-1] * max_pages for _ in range(batch)]
@@ -52,6 +63,11 @@ class PagedKV:
     def position(self, seq: int) -> int:
         return self._pos[seq]
 
+    def _check(self, seqs) -> None:
+        seqs = list(seqs)
+        if len(set(seqs)) != len(seqs) or not all(0 <= s < len(self._lens) for s in seqs):
+            raise Vx27Error(f"PagedKV: sequences {seqs} of {len(self._lens)}")
+
     def _need(self, seq: int, n: int) -> list[int]:
         """Table entries that n more slots of the sequence need a page for."""
         if n < 1:
@@ -67,8 +83,9 @@ class PagedKV:
         for s in seqs:
             self.table[s].copy_(torch.tensor(self._pages[s], dtype=torch.int32))
 
-    def _upload_lens(self) -> None:
-        self.lens.copy_(torch.tensor(self._lens, dtype=torch.int32))
+    def _upload_state(self, step: dict[int, int]) -> None:
+        one = [n if step.get(s) == 1 else 0 for s, n in enumerate(self._lens)]
+        self._state.copy_(torch.tensor([self._lens, self._pos, one], dtype=torch.int32))
 
     def _out_of_sight(self, seq: int) -> list[int]:
         """Entries that no later token attends to."""
@@ -81,7 +98,9 @@ class PagedKV:
     def extend(self, tokens: dict[int, int]) -> dict[int, tuple[int, int]]:
         """Makes room for tokens[seq] more tokens of each sequence and counts them as held:
         (first slot, first position) by sequence. Pages that earlier calls moved out of sight of
-        a window are freed first. On the device the lengths are those after these tokens."""
+        a window are freed first. On the device the state is that after these tokens; a
+        sequence that gets one token takes part in the next step_paged, the others do not."""
+        self._check(tokens)
         need = {s: self._need(s, n) for s, n in tokens.items()}
         changed = set()
         for s in tokens:
@@ -102,16 +121,17 @@ class PagedKV:
             self._lens[s] += n
             self._pos[s] += n
         self._upload(changed)
-        self._upload_lens()
+        self._upload_state(tokens)
         return at
 
     def release(self, seq: int) -> None:
         """The sequence is done: its pages are free, its lane is idle."""
+        self._check([seq])
         self._free += [p for p in self._pages[seq] if p >= 0]
         self._pages[seq] = [-1] * self.max_pages
         self._lens[seq] = self._pos[seq] = 0
         self._upload([seq])
-        self._upload_lens()
+        self._upload_state({})
         if self.sums is not None:
             self.sums[:, seq] = 0
 
@@ -124,14 +144,16 @@ class PagedKV:
         slots [layers][n][nkv][keep]."""
         if self.sums is None:
             raise Vx27Error("PagedKV: evict needs weights=True")
-        cut = [s for s in (range(len(self._lens)) if seqs is None else seqs) if self._lens[s] > keep]
+        seqs = range(len(self._lens)) if seqs is None else list(seqs)
+        self._check(seqs)
+        if not 0 <= sinks <= sinks + recent <= keep or keep < 1:
+            raise Vx27Error(f"PagedKV: keep={keep} with sinks={sinks} and recent={recent}")
+        cut = [s for s in seqs if self._lens[s] > keep]
         if not cut:
             return [], None
         n = -(-keep // self.page_size)
         if n * len(cut) > len(self._free):
             raise Vx27Error(f"PagedKV: evict needs {n * len(cut)} free pages, {len(self._free)} are")
-        if not 0 <= sinks <= sinks + recent <= keep or keep < 1:
-            raise Vx27Error(f"PagedKV: keep={keep} with sinks={sinks} and recent={recent}")
         layers, nkv, dev = len(self.k), self.k.shape[2], self.k.device
         new = [[self._free.pop() for _ in range(n)] for _ in cut]
         rows = torch.tensor(cut, device=dev)
@@ -151,7 +173,7 @@ class PagedKV:
             self._pages[s] = pages + [-1] * (self.max_pages - n)
             self._lens[s] = keep
         self._upload(cut)
-        self._upload_lens()
+        self._upload_state({})
         return cut, kept
 
     def workspace(self, nq: int) -> torch.Tensor:
