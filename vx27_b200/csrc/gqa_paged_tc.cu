@@ -802,13 +802,18 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
 }
 
 // ---- join and weight sums ---------------------------------------------------------------
-// Blocks [0, B): zeros for a sequence without slots. Then (P - 1) G blocks: (c, h) merges head h of the item that run c continues, if c is
-// the second run of it: o = sum_r w_r o_r / sum_r w_r, w_r = l_r 2^(m_r - m). The other blocks
-// add the weights of 1024 slots of an item: sum_h 2^(s_h - m_h) / l_h.
-__global__ void __launch_bounds__(256)
+// Blocks [0, B): zeros for a sequence without slots. Then (P - 1) G blocks: (c, h) merges head
+// h of the item that run c continues, if c is the second run of it: o = sum_r w_r o_r / sum_r
+// w_r, w_r = l_r 2^(m_r - m). The other blocks add the weights of 1024 slots of an item: sum_h
+// 2^(s_h - m_h) / l_h.
+// Nothing but round trips and instructions bound it. The first two records of an item are those
+// of runs c - 1 and c, so they are requested along with the plan; RU records a round
+// trip: 40 where runs share items (FEW: the batch has fewer items than half the runs), else 4.
+template <bool FEW>
+__global__ void __launch_bounds__(256, FEW ? 3 : 5)
 paged_join_k(const __grid_constant__ DecodeArgs a, int P, int G, int slot_blocks) {
     grid_dep_wait();
-    __shared__ float w_s[JOIN_MAX], red[8];
+    __shared__ float w_s[JOIN_MAX];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int n_join = (P - 1) * G, blk = (int)blockIdx.x - a.B;
     if (blk < 0) {
@@ -822,46 +827,52 @@ paged_join_k(const __grid_constant__ DecodeArgs a, int P, int G, int slot_blocks
     }
     // records of runs c1 .. c2: the first is that run's last item, the others first items
     auto rec_of = [](int c1, int r) { return (size_t)(r == 0 ? 2 * c1 + 1 : 2 * (c1 + r)); };
-    auto block_max = [&](float m) {
-        m = warp_max(m);
-        __syncthreads();
-        if (lane == 0) red[warp] = m;
-        __syncthreads();
-        float t = red[0];
-        for (int i = 1; i < 8; i++) t = fmaxf(t, red[i]);
-        return t;
-    };
     if (blk < n_join) {
-        const int4 j = a.join[blk / G + 1];
-        const int h = blk % G;
+        const int c = blk / G + 1, h = blk % G;
+        const float *ro = a.rec_o + (size_t)(2 * c - 1) * G * HD + h * HD + tid;
+        const float2 *rm = a.rec_ml + (size_t)(2 * c - 1) * G + h;
+        const float v0 = ro[0], v1 = ro[G * HD];
+        const float2 ml0 = rm[0], ml1 = rm[G];
+        const int4 j = a.join[c];
         if (j.x < 0) return;
-        const int c1 = j.y, n = j.z - j.y + 1;
-        // one round trip: the gate, the (m, l) and the column's first values are requested together
+        const int n = j.z - j.y + 1;
         const size_t i = ((size_t)(j.x / a.pool.nkv) * a.nq + (j.x % a.pool.nkv) * G + h) * HD + tid;
         const float g = !a.gate ? 0.f : a.gate_bf16 ? act_ld<true>(a.gate, i) : act_ld<false>(a.gate, i);
-        constexpr int RU = 40;
-        float v[RU];
+        float L, O;
+        if (n == 2) {
+            const float m = fmaxf(ml0.x, ml1.x);
+            const float w0 = ml0.y * exp2f(ml0.x - m), w1 = ml1.y * exp2f(ml1.x - m);
+            L = w0 + w1;
+            O = fmaf(w1, v1, w0 * v0);
+        } else {
+            constexpr int RU = FEW ? 38 : 4;
+            ro += (size_t)G * HD;  // record r >= 1 of the item is at 2 (r - 1) records from here
+            rm += G;
+            float v[RU];
 #pragma unroll
-        for (int u = 0; u < RU; u++)
-            v[u] = u < n ? a.rec_o[(rec_of(c1, u) * G + h) * HD + tid] : 0.f;
-        float m = -INFINITY;
-        for (int r = tid; r < n; r += 256) m = fmaxf(m, a.rec_ml[rec_of(c1, r) * G + h].x);
-        m = block_max(m);
-        for (int r = tid; r < n; r += 256) {
-            const float2 ml = a.rec_ml[rec_of(c1, r) * G + h];
-            w_s[r] = ml.y * exp2f(ml.x - m);
-        }
-        __syncthreads();
-        float L = 0.f, O = 0.f;
+            for (int u = 0; u < RU; u++) v[u] = u + 2 < n ? ro[(u + 1) * 2 * G * HD] : 0.f;
+            float m = fmaxf(ml0.x, ml1.x);  // every warp makes it
+            for (int r = 2 + lane; r < n; r += 32) m = fmaxf(m, rm[(size_t)(r - 1) * 2 * G].x);
+            m = warp_max(m);
+            for (int r = 2 + tid; r < n; r += 256) {
+                const float2 ml = rm[(size_t)(r - 1) * 2 * G];
+                w_s[r] = ml.y * exp2f(ml.x - m);
+            }
+            const float w0 = ml0.y * exp2f(ml0.x - m), w1 = ml1.y * exp2f(ml1.x - m);
+            L = w0 + w1;
+            O = fmaf(w1, v1, w0 * v0);
+            __syncthreads();
 #pragma unroll
-        for (int u = 0; u < RU; u++) {
-            const float wr = u < n ? w_s[u] : 0.f;
-            L += wr;
-            O = fmaf(wr, v[u], O);
-        }
-        for (int r = RU; r < n; r++) {
-            L += w_s[r];
-            O = fmaf(w_s[r], a.rec_o[(rec_of(c1, r) * G + h) * HD + tid], O);
+            for (int u = 0; u < RU; u++) {
+                const float wr = u + 2 < n ? w_s[u + 2] : 0.f;
+                L += wr;
+                O = fmaf(wr, v[u], O);
+            }
+#pragma unroll 4
+            for (int r = RU + 2; r < n; r++) {
+                L += w_s[r];
+                O = fmaf(w_s[r], ro[(size_t)(r - 1) * 2 * G * HD], O);
+            }
         }
         float o = O / L;
         if (a.gate) o *= 1.0f / (1.0f + expf(-g));
@@ -992,7 +1003,9 @@ int launch_paged_decode(const DecodeArgs &a, const void *k_pages, const void *v_
     }
 #undef VX_G
 #undef VX_D
-    VX_CK(launch_pdl(paged_join_k, dim3((unsigned)blocks), dim3(256), 0, st, a, P, G, slot_blocks));
+    const bool few = 2LL * a.B * a.pool.nkv < P;
+    VX_CK(launch_pdl(few ? paged_join_k<true> : paged_join_k<false>, dim3((unsigned)blocks), dim3(256), 0, st,
+                     a, P, G, slot_blocks));
     return 0;
 }
 
