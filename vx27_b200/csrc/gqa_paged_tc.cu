@@ -27,8 +27,8 @@
 // the other groups out; unseen rows of a copied group are zeroed.
 //
 // Warps: 0 copies K and 7 copies V (lane i: rows 16 i .. of the tile; page ids come a tile
-// ahead), 1 issues the S MMAs and 8 the O MMAs, 2-5 softmax and accumulation, 6 q, gate and
-// results. Waits are bounded (2 s).
+// ahead), 1 issues the S MMAs and 8 the O MMAs, 2-5 softmax and accumulation, 6 q, 9-11 gate
+// and results. Waits are bounded (2 s).
 #include <math.h>
 #include <algorithm>
 #include "common.cuh"
@@ -43,8 +43,9 @@ constexpr int HD = PG_HD;
 constexpr int TILE = 128;
 constexpr int NK = 6, NV = 6;      // ring slots; NV even: a V operand is two neighbouring chunks
 constexpr int CHUNK = 16384;       // 128 slots x 64 dims, 128-byte swizzle
-constexpr int THREADS = 288;
-constexpr int SM_WARP0 = 2, STAGE_WARP = 6, V_WARP = 7, O_WARP = 8;  // 0: K copies, 1: S MMAs
+constexpr int THREADS = 384;
+constexpr int SM_WARP0 = 2, Q_WARP = 6, V_WARP = 7, O_WARP = 8;  // 0: K copies, 1: S MMAs
+constexpr int OUT_WARP0 = 9, OUT_WARPS = 3;
 constexpr int JOIN_MAX = 1024;     // runs at most (records of one item)
 constexpr int RUN_LENS = 128;      // lengths kept in shared memory
 
@@ -261,7 +262,7 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
             mbar_init(&sm.q_empty[i], 1);
         }
         mbar_init(&sm.ob_full, 128);
-        mbar_init(&sm.ob_empty, 1);
+        mbar_init(&sm.ob_empty, OUT_WARPS);
         mbar_init(&sm.mma_done[0], 1);
         mbar_init(&sm.mma_done[1], 1);
         sm.abort = 0;
@@ -275,7 +276,7 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
             tma_prefetch_desc(&tmv);
         }
     }
-    if (warp >= SM_WARP0 && warp < STAGE_WARP) {  // operand rows that no term fills stay zero
+    if (warp >= SM_WARP0 && warp < Q_WARP) {  // operand rows that no term fills stay zero
         uint4 *z = reinterpret_cast<uint4 *>(&sm.q[0][0][0]);
         for (int e = tid - 64; e < (int)(sizeof(sm.q) + sizeof(sm.p)) / 16; e += 128)
             z[e] = make_uint4(0, 0, 0, 0);
@@ -543,7 +544,7 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
             mma_commit(&sm.mma_done[1]);
             bar_drain(&sm.mma_done[1], 0);
         }
-    } else if (warp < STAGE_WARP) {
+    } else if (warp < Q_WARP) {
         // ---- softmax: thread = slot r of the tile; then output dims r and r + 128 ----------
         const int q4 = warp & 3, r = q4 * 32 + lane;
         const uint32_t lane_addr = tmem + ((uint32_t)(q4 * 32) << 16);
@@ -693,20 +694,30 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
                 w.next();
             }
         }
-    } else {
-        // ---- q in, results out --------------------------------------------------------------
-        if (start.done() && lane == 0) a.join[c] = make_int4(-1, 0, 0, 0);
+    } else if (warp == Q_WARP) {
+        // ---- q, split into terms --------------------------------------------------------------
+        if (lane == 0) {
+            // an item that began in an earlier run is joined by the block of its second run
+            int4 j = make_int4(-1, 0, 0, 0);
+            if (!start.done() && start.v0 > 0) {
+                const int c1 = owner(begin - start.v0), c2 = owner(begin - start.v0 + start.t.tiles - 1);
+                if (c == c1 + 1) j = make_int4(start.b * nkv + start.h, c1, c2, 0);
+            }
+            a.join[c] = j;
+        }
+        const int d0 = 8 * lane;
         bool ok = true;
         int kq = 0;
-        const int d0 = 8 * lane;
-        float qv[G][8];
-        auto load_q = [&](const Walk &w) {
+        for (Walk w = start; !w.done(); w.next(), kq++) {
+            float x[G][8];
 #pragma unroll
             for (int h = 0; h < G; h++)
-                ld8_f32(qv[h], a.q + ((size_t)w.b * a.nq + w.h * G + h) * HD + d0);
-        };
-        auto store_q = [&](int qb) {  // split into terms
-            uint8_t *dst = sm.q[qb][d0 >> 6];
+                ld8_f32(x[h], a.q + ((size_t)w.b * a.nq + w.h * G + h) * HD + d0);
+            if (kq >= QB)  // the S MMAs of the item that used the buffer before are complete
+                ok = bar_wait(&sm.q_empty[kq % QB], ((kq - QB) / QB) & 1, &sm.abort, status,
+                              VX_DEV_TIMEOUT_MMA);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            uint8_t *dst = sm.q[kq % QB][d0 >> 6];
 #pragma unroll
             for (int h = 0; h < G; h++)
 #pragma unroll
@@ -714,83 +725,69 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
                     uint32_t wd[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        wd[e] = pack_bf16x2(qv[h][2 * e], qv[h][2 * e + 1]);
-                        qv[h][2 * e] -= bf16_to_f32(wd[e] & 0xffffu);
-                        qv[h][2 * e + 1] -= bf16_to_f32(wd[e] >> 16);
+                        wd[e] = pack_bf16x2(x[h][2 * e], x[h][2 * e + 1]);
+                        x[h][2 * e] -= bf16_to_f32(wd[e] & 0xffffu);
+                        x[h][2 * e + 1] -= bf16_to_f32(wd[e] >> 16);
                     }
                     *reinterpret_cast<uint4 *>(dst + sw128(h + k * G, d0 & 63)) =
                         make_uint4(wd[0], wd[1], wd[2], wd[3]);
                 }
             fence_proxy_async();
-            mbar_arrive(&sm.q_full[qb]);
-        };
-        Walk nx = start, w = start;  // the item whose q is staged next; whose result is due
-        for (int kn = 0; ok;) {      // kn items staged: this one's and the next one's q, then its result
-            if (kn <= kq + 1 && !nx.done()) {
-                load_q(nx);
-                if (kn >= QB)  // the S MMAs of the item that used the buffer before are complete
-                    ok = bar_wait(&sm.q_empty[kn % QB], ((kn - QB) / QB) & 1, &sm.abort, status,
-                                  VX_DEV_TIMEOUT_MMA);
-                ok = __all_sync(0xffffffffu, ok);
-                if (ok) store_q(kn % QB);
-                nx.next();
-                if (kn++ == 0 && lane == 0) {
-                    // an item that began in an earlier run is joined by the block of its second run
-                    int4 j = make_int4(-1, 0, 0, 0);
-                    if (w.v0 > 0) {
-                        const int c1 = owner(begin - w.v0), c2 = owner(begin - w.v0 + w.t.tiles - 1);
-                        if (c == c1 + 1) j = make_int4(w.b * nkv + w.h, c1, c2, 0);
-                    }
-                    a.join[c] = j;
-                }
-                continue;
-            }
-            if (w.done()) break;
+            mbar_arrive(&sm.q_full[kq % QB]);
+        }
+    } else {
+        // ---- results: warp OUT_WARP0 + i has heads i, i + OUT_WARPS, .. of the group -----------
+        constexpr int HW = (G + OUT_WARPS - 1) / OUT_WARPS;
+        const int h0 = warp - OUT_WARP0, d0 = 8 * lane;
+        bool ok = true;
+        int kq = 0;
+        for (Walk w = start; !w.done(); w.next(), kq++) {
             const size_t base = ((size_t)w.b * a.nq + w.h * G) * HD + d0;
             const bool whole = w.whole();
-            float gv[G][8];
+            float gv[HW][8], o[HW][8];
             if (whole && a.gate) {
 #pragma unroll
-                for (int h = 0; h < G; h++) {
-                    if (a.gate_bf16) ld8_bf16(gv[h], static_cast<const uint16_t *>(a.gate) + base + h * HD);
-                    else ld8_f32(gv[h], static_cast<const float *>(a.gate) + base + h * HD);
+                for (int u = 0; u < HW; u++) {
+                    const int h = h0 + u * OUT_WARPS;
+                    if (h >= G) break;
+                    if (a.gate_bf16) ld8_bf16(gv[u], static_cast<const uint16_t *>(a.gate) + base + h * HD);
+                    else ld8_f32(gv[u], static_cast<const float *>(a.gate) + base + h * HD);
                 }
             }
-            ok = ok && bar_wait(&sm.ob_full, kq & 1, &sm.abort, status, VX_DEV_TIMEOUT_MMA);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
+            ok = bar_wait(&sm.ob_full, kq & 1, &sm.abort, status, VX_DEV_TIMEOUT_MMA);
+            if (!__all_sync(0xffffffffu, ok)) break;
             // the buffer is free once it is in registers (an arrival after the global stores
             // waits for them)
-            float o[G][8];
 #pragma unroll
-            for (int h = 0; h < G; h++) ld8_f32(o[h], &sm.ob[h][d0]);
+            for (int u = 0; u < HW; u++)
+                if (h0 + u * OUT_WARPS < G) ld8_f32(o[u], &sm.ob[h0 + u * OUT_WARPS][d0]);
             const float2 ml = lane < G ? make_float2(sm.ml[lane][0], sm.ml[lane][1]) : make_float2(0, 0);
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.ob_empty);
             const size_t rec = (size_t)(2 * c + (w.v0 > 0 ? 0 : 1)) * G;
             const int item = w.b * nkv + w.h;
 #pragma unroll
-            for (int h = 0; h < G; h++) {
+            for (int u = 0; u < HW; u++) {
+                const int h = h0 + u * OUT_WARPS;
+                if (h >= G) break;
                 if (!whole) {
-                    st8_f32(a.rec_o + (rec + h) * HD + d0, o[h]);
+                    st8_f32(a.rec_o + (rec + h) * HD + d0, o[u]);
                 } else {
                     if (a.gate)
 #pragma unroll
                         for (int e = 0; e < 8; e++)
-                            o[h][e] *= __fdividef(1.0f, 1.0f + __expf(-gv[h][e]));
-                    if (a.out_bf16) st8_bf16(static_cast<uint16_t *>(a.out) + base + h * HD, o[h]);
-                    else st8_f32(static_cast<float *>(a.out) + base + h * HD, o[h]);
+                            o[u][e] *= __fdividef(1.0f, 1.0f + __expf(-gv[u][e]));
+                    if (a.out_bf16) st8_bf16(static_cast<uint16_t *>(a.out) + base + h * HD, o[u]);
+                    else st8_f32(static_cast<float *>(a.out) + base + h * HD, o[u]);
                 }
             }
-            if (lane < G) {
+            if (h0 == 0 && lane < G) {
                 if (!whole) a.rec_ml[rec + lane] = ml;
                 else if (a.scores) a.item_ml[(size_t)item * G + lane] = ml;
             }
             // which runs hold the item, for the weight sums
-            if (lane == 0 && a.scores && w.v0 == 0)
+            if (h0 == 0 && lane == 0 && a.scores && w.v0 == 0)
                 a.span[item] = make_int2(c, owner(end - w.left + w.t.tiles - 1));
-            w.next();
-            kq++;
         }
     }
     __syncwarp();
