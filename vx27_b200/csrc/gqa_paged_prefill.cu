@@ -674,20 +674,29 @@ prompt_join_k(const __grid_constant__ PromptArgs a) {
         if (t0 + r >= a.T) return;
         // parts: the item begins in run c - 1 (its last), runs c .. c2 go on with it (their first)
         auto row = [&](int i) { return (size_t)((2 * i + (i < c ? 1 : 0)) * 2 + rank) * QT + r; };
-        float m = -INFINITY, l = 0.f, o[8] = {};
-        for (int i = c - 1; i <= c2; i++) m = fmaxf(m, a.rec_ml[row(i)].x);
-        for (int i = c - 1; i <= c2; i++) {
+        // the first two parts' rows and the gate in one round trip
+        const size_t at = ((size_t)(t0 + r) * a.nq + h) * HD + 8 * lane, r0 = row(c - 1), r1 = row(c);
+        float o[8], x[8], gate[8];
+        ld8_f32(o, a.rec_o + r0 * HD + 8 * lane);
+        ld8_f32(x, a.rec_o + r1 * HD + 8 * lane);
+        if (a.gate) ld8_bf16(gate, a.gate + at);
+        const float2 ml0 = a.rec_ml[r0], ml1 = a.rec_ml[r1];
+        float m = fmaxf(ml0.x, ml1.x);
+        for (int i = c + 1; i <= c2; i++) m = fmaxf(m, a.rec_ml[row(i)].x);
+        // a part without a seen slot has m = -inf (and l = 0)
+        const float f0 = ml0.x == -INFINITY ? 0.f : exp2f(ml0.x - m);
+        const float f1 = ml1.x == -INFINITY ? 0.f : exp2f(ml1.x - m);
+        float l = fmaf(ml1.y, f1, ml0.y * f0);
+#pragma unroll
+        for (int e = 0; e < 8; e++) o[e] = fmaf(x[e], f1, o[e] * f0);
+        for (int i = c + 1; i <= c2; i++) {
             const float2 ml = a.rec_ml[row(i)];
-            const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);  // a part without a seen slot
-            float x[8];
+            const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
             ld8_f32(x, a.rec_o + row(i) * HD + 8 * lane);
             l = fmaf(ml.y, f, l);
 #pragma unroll
             for (int e = 0; e < 8; e++) o[e] = fmaf(x[e], f, o[e]);
         }
-        const size_t at = ((size_t)(t0 + r) * a.nq + h) * HD + 8 * lane;
-        float gate[8];
-        if (a.gate) ld8_bf16(gate, a.gate + at);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             o[e] /= l;

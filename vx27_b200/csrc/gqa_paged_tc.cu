@@ -18,10 +18,14 @@
 //
 // What bounds it: the cache bytes, 128 KB per tile through two rings of 6 chunks of 16 KB (128
 // slots x 64 dims) per SM, one for K and one for V, each with a copying and a multiplying warp
-// of its own. 128 sequences of 2048 slots (1.07 GB) take 179-183 us, 0.89-0.915 of the copy
+// of its own. 128 sequences of 2112 slots (1.1 GB) take 179-182 us, 0.926-0.94 of the copy
 // rate (0.84 with one ring, one copying and one multiplying warp, where a wait for K holds up
-// V). A small batch is bound by its chain instead: start and scan of the lengths 1.5 us,
-// first data 5, last result 2, join 3.5.
+// V); 128 ragged ones 178. About 15 us of a call are its ends, whatever the size: the scan of
+// the lengths 2 us, the first data 4, the last tile's products and rows 4, the join 3, and
+// with the memory busy the last CTA ends 4-8% after the middle one. (Handing the last 3-8% of the
+// tiles out late, to CTAs that start where others end, cost more than that: 107 us instead of 99
+// for 64 sequences.) Short sequences are bound by the chain of each item through the warps:
+// 256 of 100 slots take 38 us (48 with q and the results in one warp).
 // A page is a box of its own: boxes of min(page_size, 128) rows where all of them are seen,
 // else boxes of the 16-row groups with a seen slot. The O MMAs take 16 slots each and leave
 // the other groups out; unseen rows of a copied group are zeroed.
@@ -804,8 +808,10 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
 // w_r, w_r = l_r 2^(m_r - m). The other blocks add the weights of 1024 slots of an item: sum_h
 // 2^(s_h - m_h) / l_h.
 // Nothing but round trips and instructions bound it. The first two records of an item are those
-// of runs c - 1 and c, so they are requested along with the plan; RU records a round
-// trip: 40 where runs share items (FEW: the batch has fewer items than half the runs), else 4.
+// of runs c - 1 and c, so they are requested along with the plan. Items of more records take 38
+// more of them per round trip (FEW: at most an eighth as many items as runs) or 4, in
+// fewer registers: one sequence of 8192 slots (37 runs an item) takes 20.8 us in all with FEW and
+// 24.2 without, 4 of them 34.5 and 34.6, 8 of 2112 25.0 and 24.5, 16 of them 37.1 and 36.3.
 template <bool FEW>
 __global__ void __launch_bounds__(256, FEW ? 3 : 5)
 paged_join_k(const __grid_constant__ DecodeArgs a, int P, int G, int slot_blocks) {
@@ -1000,7 +1006,7 @@ int launch_paged_decode(const DecodeArgs &a, const void *k_pages, const void *v_
     }
 #undef VX_G
 #undef VX_D
-    const bool few = 2LL * a.B * a.pool.nkv < P;
+    const bool few = 8LL * a.B * a.pool.nkv < P;
     VX_CK(launch_pdl(few ? paged_join_k<true> : paged_join_k<false>, dim3((unsigned)blocks), dim3(256), 0, st,
                      a, P, G, slot_blocks));
     return 0;
