@@ -1,8 +1,8 @@
 /*
  * libvx27cuda -- B200 (sm_100a) implementation of the vx27 attention hot path.
  *
- * Library-wide definitions shared by vx27_deltanet.h, vx27_gqa.h, vx27_kv.h and
- * vx27_rope.h. The reference (DavidPandleton/vx27) has no counterpart for this header:
+ * Library-wide definitions shared by vx27_deltanet.h, vx27_gqa.h, vx27_kv.h, vx27_paged.h
+ * and vx27_rope.h. The reference (DavidPandleton/vx27) has no counterpart for this header:
  * its hot-path functions return void and report nothing (src/vx27_deltanet.h:10-59).
  *
  * Two tiers share this library:
