@@ -57,7 +57,8 @@ int vx27_gqa_paged_append(const void *q_in, const void *k_in, const void *v_in,
  * Attention of one token per sequence over the lens[b] slots that the sequence holds (the
  * token's own is the last), or those of them in the window: out = softmax(q k^T / sqrt(hd)) v
  * * sigmoid(gate) per query head (head h reads KV head h * nkv / nq). lens[b] = 0: a row of
- * zeros. What lies in masked slots, NaN and infinities among it, has no effect.
+ * zeros. What lies in masked slots, NaN and infinities among it, has no effect; seen K and V rows
+ * and q are finite (an infinity among them gives NaN, since q is split into terms).
  *   q [B][nq][hd] fp32; gate [B][nq][hd] (act dtype) or NULL; out [B][nq][hd] (fp32, or bf16
  *   with VX27_F_OUT_BF16)
  *   weight_sum fp32 [B][nkv][max_pages * page_size] or NULL: to the entry of each slot attended

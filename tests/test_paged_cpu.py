@@ -228,3 +228,12 @@ def test_paged_cache_refusals():
         with pytest.raises(ops.Vx27Error, match="sequences"):
             c.evict(20, seqs=bad)
     held(c)
+
+
+def test_layer_refuses_a_prompt_without_room():
+    from vx27_b200.layer import GQALayer
+    layer, c = object.__new__(GQALayer), cache()
+    c.extend({1: 20})
+    for seq, slot, n in ((1, 0, 21), (1, 15, 6), (1, -1, 5), (0, 0, 1), (-1, 0, 1)):
+        with pytest.raises(ops.Vx27Error, match="prompt_paged"):
+            layer.prompt_paged(torch.zeros(n, 8), c, 0, seq, slot, slot, None)

@@ -147,6 +147,9 @@ class GQALayer:
         """T prompt tokens of one sequence of a paged.PagedKV, whose extend() has made room for
         them at (slot, pos): x [T, H] fp32. The attention runs in bf16. Returns [T, H] fp32."""
         T = x.shape[0]
+        if seq < 0 or slot < 0 or slot + T > cache.length(seq):
+            raise ops.Vx27Error(f"prompt_paged: {T} tokens from slot {slot}, sequence {seq} holds "
+                                f"{cache.length(seq)}")
         q_in, gate, k, v = self._project(x, None)
         at = torch.arange(T, dtype=torch.int32, device=x.device)
         q = torch.empty(q_in.shape, dtype=torch.bfloat16, device=x.device)

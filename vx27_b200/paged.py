@@ -33,7 +33,8 @@ class PagedKV:
                  weights: bool = False, device="cuda"):
         """n_pages pages for batch sequences of at most max_pages pages each. window, sinks: what
         every token attends to (0: everything); pages that fall out of sight are freed. weights:
-        the attention each slot gets is summed, for evict."""
+        the attention each slot gets from the tokens of step_paged is summed, for evict (a
+        prompt's tokens add nothing)."""
         if window < 0 or sinks < 0 or (sinks and not window):
             raise Vx27Error(f"PagedKV: window={window} with sinks={sinks}")
         if weights and window:
