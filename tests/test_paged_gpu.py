@@ -148,6 +148,28 @@ def test_decode_ragged(cuda, ps, out, n_parts):
     assert (got[0] == 0).all()
 
 
+@pytest.mark.parametrize("weights", [False, True])
+def test_decode_many_sequences(cuda, weights):
+    """More sequences than a CTA has threads, long stretches of idle ones in a run; then all idle."""
+    g = gen(6)
+    B = 1500
+    lens = [0 if 300 <= b < 800 or b % 7 == 0 else 1 + b * 37 % 150 for b in range(B)]
+    lens[600], lens[-1] = 700, 0
+    pool = Pool(g, lens, 2, 16)
+    q = normal(g, B, 4, HD)
+    w = torch.zeros(B, 2, pool.max_pages * 16, device="cuda") if weights else None
+    got = run_decode(pool, q, None, lens, torch.float32, weights=w)
+    ref, tol, sums, stol = decode_ref(pool, q, None, lens, 0, 0, False, True)
+    close(got, ref, tol)
+    assert (got[torch.tensor(lens) == 0] == 0).all()
+    if weights:
+        close(w, sums, stol)
+    got = run_decode(pool, q, None, [0] * B, BF, weights=w)
+    assert (got == 0).all()
+    if weights:
+        close(w, sums, stol)
+
+
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (16, 4), (100, 4), (128, 130), (129, 1),
                                           (300, 0), (5000, 4)])
 @pytest.mark.parametrize("ps,n_parts", [(16, 0), (64, 2), (256, 1)])
@@ -449,6 +471,40 @@ def test_prompt_few_rows_over_many_slots(cuda, nq, nkv, T, s0, window, sinks):
     for gt in (gate, None):
         got = run_prompt(pool, q, gt, s0, window, sinks)
         close(got, *prompt_ref(pool, q, gt, s0, window, sinks))
+
+
+def test_prompts_replay_and_overlap(cuda):
+    """Two captured prompts (one of them joined from parts), replayed at once on streams and
+    workspaces of their own with other rows in the same buffers; a table row that is not the first."""
+    g = gen(24)
+    cases = []
+    for T, s0, b in ((200, 100, 0), (3, 5000, 1)):
+        pool = Pool(g, [40, s0 + T] if b else [s0 + T, 40], 4, 64)
+        q, gate = normal(g, T, 24, HD).to(BF), normal(g, T, 24, HD).to(BF)
+        out = torch.empty_like(q)
+        ws = torch.empty(ops.gqa_paged_prefill_workspace_bytes(4, HD), dtype=torch.uint8, device="cuda")
+
+        def call(pool=pool, q=q, gate=gate, out=out, ws=ws, s0=s0, b=b):
+            ops.gqa_paged_prefill(q, gate, pool.k, pool.v, pool.table[b], out, ws, s0=s0)
+        call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call()
+        cases.append((pool, q, gate, out, s0, b, graph, torch.cuda.Stream()))
+    for pool, q, gate, out, *_ in cases:
+        q.copy_(normal(g, *q.shape))
+        out.fill_(float("nan"))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for *_, graph, stream in cases:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert ops.device_status() == 0
+    for pool, q, gate, out, s0, b, *_ in cases:
+        pool.table = pool.table[b:].clone()  # of prompt_ref's sequence 0
+        close(out, *prompt_ref(pool, q, gate, s0, 0, 0))
 
 
 def test_prompt_bad_page_is_reported(cuda):
