@@ -66,6 +66,7 @@ WINDOW = [(dict(window=-1), "window=-1"), (dict(window=4, sinks=-1), "sinks=-1")
         (dict(q=P(8)), "16-byte aligned"), (dict(slots=None), "null pointer")]),
     ("vx27_gqa_paged_decode", _decode, POOL + HEADS + WINDOW + [
         (dict(B=0), "B=0"), (dict(B=65536), "B=65536"), (dict(lens=None), "null pointer"),
+        (dict(wsum=P(8)), "16-byte aligned"),
         (dict(ws=None), "null pointer"), (dict(wsb=0), "workspace of 0 bytes"),
         (dict(out=P(24)), "16-byte aligned")]),
     ("vx27_gqa_paged_prefill", _prefill, POOL + HEADS + WINDOW + [

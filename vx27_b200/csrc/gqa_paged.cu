@@ -257,8 +257,9 @@ int vx27_gqa_paged_decode(const float *q, const void *gate, const void *k_pages,
         return -1;
     if (B <= 0 || B > 65535) return fail(err, errlen, "%s: B=%d", fn, B);
     if (!q || !lens || !out || !workspace) return fail(err, errlen, "%s: null pointer argument", fn);
-    if (((uintptr_t)q | (uintptr_t)gate | (uintptr_t)out | (uintptr_t)workspace) & 15)
-        return fail(err, errlen, "%s: q, gate, out and the workspace must be 16-byte aligned", fn);
+    if (((uintptr_t)q | (uintptr_t)gate | (uintptr_t)out | (uintptr_t)workspace | (uintptr_t)weight_sum) & 15)
+        return fail(err, errlen, "%s: q, gate, out, weight_sum and the workspace must be 16-byte aligned",
+                    fn);
     DecodeArgs a{};
     int P = paged_decode_parts(n_parts);
     const size_t need = paged_decode_layout(a, workspace, B, nq, nkv, max_pages * page_size, window,

@@ -18,9 +18,9 @@
 //
 // What bounds it: the cache bytes, 128 KB per tile through two rings of 6 chunks of 16 KB (128
 // slots x 64 dims) per SM, one for K and one for V, each with a copying and a multiplying warp
-// of its own. 128 sequences of 2112 slots (1.1 GB) take 179-182 us, 0.926-0.94 of the copy
+// of its own. 128 sequences of 2112 slots (1.1 GB) take 177-180 us, 0.94-0.95 of the copy
 // rate (0.84 with one ring, one copying and one multiplying warp, where a wait for K holds up
-// V); 128 ragged ones 178. About 15 us of a call are its ends, whatever the size: the scan of
+// V); 128 ragged ones 174. About 15 us of a call are its ends, whatever the size: the scan of
 // the lengths 2 us, the first data 4, the last tile's products and rows 4, the join 3, and
 // with the memory busy the last CTA ends 4-8% after the middle one. (Handing the last 3-8% of the
 // tiles out late, to CTAs that start where others end, cost more than that: 107 us instead of 99
@@ -812,8 +812,11 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
 // more of them per round trip (FEW: at most an eighth as many items as runs) or 4, in
 // fewer registers: one sequence of 8192 slots (37 runs an item) takes 20.8 us in all with FEW and
 // 24.2 without, 4 of them 34.5 and 34.6, 8 of 2112 25.0 and 24.5, 16 of them 37.1 and 36.3.
-template <bool FEW>
-__global__ void __launch_bounds__(256, FEW ? 3 : 5)
+// WEIGHTS is an instance of its own, whose registers the others need not have; sums are read and
+// written four at a time, requested with the scores (32 ragged sequences 62.5 us in all, 65.7
+// with scalar sums added at the end, 56 without sums).
+template <bool FEW, bool WEIGHTS>
+__global__ void __launch_bounds__(256, FEW ? 3 : WEIGHTS ? 4 : 5)
 paged_join_k(const __grid_constant__ DecodeArgs a, int P, int G, int slot_blocks) {
     grid_dep_wait();
     __shared__ float w_s[JOIN_MAX];
@@ -883,18 +886,24 @@ paged_join_k(const __grid_constant__ DecodeArgs a, int P, int G, int slot_blocks
         else act_st<false>(a.out, i, o);
         return;
     }
-    // 4 slots a thread; the scores are requested before the statistics, which warp h makes for
-    // head h
+    if constexpr (!WEIGHTS) return;
+    // 4 slots a thread; their scores and sums are requested before the statistics, which warp h
+    // makes for head h
     const int bi = blk - n_join, item = bi / slot_blocks, k0 = (bi % slot_blocks) * 1024 + 4 * tid;
     const SeqTiles t(seq_len(a, item / a.pool.nkv), a.window, a.sinks);
     if ((bi % slot_blocks) * 1024 >= t.tiles * TILE) return;
+    const int slot = t.first_slot(k0 / TILE) + k0 % TILE;
+    const bool seen[4] = {t.see.sees(slot), t.see.sees(slot + 1), t.see.sees(slot + 2), t.see.sees(slot + 3)};
+    const bool any = k0 < t.tiles * TILE && (seen[0] || seen[1] || seen[2] || seen[3]);
     const float *sc = a.scores + (size_t)item * G * a.score_stride + k0;
+    float4 *ws = reinterpret_cast<float4 *>(a.wsum + (size_t)item * ((size_t)a.max_pages << a.pool.ps_log) +
+                                            slot);
+    const float4 old = any ? *ws : make_float4(0, 0, 0, 0);
     float4 x[8];
 #pragma unroll
     for (int h = 0; h < 8; h++)
-        x[h] = h < G && k0 < t.tiles * TILE
-                   ? *reinterpret_cast<const float4 *>(sc + (size_t)h * a.score_stride)
-                   : make_float4(0, 0, 0, 0);
+        x[h] = h < G && any ? *reinterpret_cast<const float4 *>(sc + (size_t)h * a.score_stride)
+                            : make_float4(0, 0, 0, 0);
     __shared__ float2 ml_s[8];
     if (warp < G) {
         const int2 span = a.span[item];
@@ -925,13 +934,9 @@ paged_join_k(const __grid_constant__ DecodeArgs a, int P, int G, int slot_blocks
         sum.z = fmaf(exp2f(x[h].z - ml.x), ml.y, sum.z);
         sum.w = fmaf(exp2f(x[h].w - ml.x), ml.y, sum.w);
     }
-    if (k0 >= t.tiles * TILE) return;
-    const int slot = t.first_slot(k0 / TILE) + k0 % TILE;
-    float *ws = a.wsum + (size_t)item * ((size_t)a.max_pages << a.pool.ps_log) + slot;
-    if (t.see.sees(slot)) ws[0] += sum.x;
-    if (t.see.sees(slot + 1)) ws[1] += sum.y;
-    if (t.see.sees(slot + 2)) ws[2] += sum.z;
-    if (t.see.sees(slot + 3)) ws[3] += sum.w;
+    if (any)
+        *ws = make_float4(seen[0] ? old.x + sum.x : old.x, seen[1] ? old.y + sum.y : old.y,
+                          seen[2] ? old.z + sum.z : old.z, seen[3] ? old.w + sum.w : old.w);
 }
 
 }  // namespace
@@ -1007,8 +1012,9 @@ int launch_paged_decode(const DecodeArgs &a, const void *k_pages, const void *v_
 #undef VX_G
 #undef VX_D
     const bool few = 8LL * a.B * a.pool.nkv < P;
-    VX_CK(launch_pdl(few ? paged_join_k<true> : paged_join_k<false>, dim3((unsigned)blocks), dim3(256), 0, st,
-                     a, P, G, slot_blocks));
+    auto join = a.scores ? (few ? paged_join_k<true, true> : paged_join_k<false, true>)
+                         : (few ? paged_join_k<true, false> : paged_join_k<false, false>);
+    VX_CK(launch_pdl(join, dim3((unsigned)blocks), dim3(256), 0, st, a, P, G, slot_blocks));
     return 0;
 }
 
