@@ -22,7 +22,8 @@
  * is then read or written, and the results of that sequence are unspecified.
  *
  * All calls enqueue on the stream and return; they allocate nothing and may be captured
- * into a graph. Calls that overlap on the GPU need workspaces of their own.
+ * into a graph, which keeps the addresses: tables, lengths, caches and workspace live as long
+ * as it does. Calls that overlap on the GPU need workspaces of their own.
  */
 #ifndef VX27_PAGED_H
 #define VX27_PAGED_H

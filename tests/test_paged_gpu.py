@@ -491,7 +491,7 @@ def test_prompts_replay_and_overlap(cuda):
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             call()
-        cases.append((pool, q, gate, out, s0, b, graph, torch.cuda.Stream()))
+        cases.append((pool, q, gate, out, s0, b, ws, graph, torch.cuda.Stream()))
     for pool, q, gate, out, *_ in cases:
         q.copy_(normal(g, *q.shape))
         out.fill_(float("nan"))
