@@ -33,3 +33,28 @@ def test_paged_rows_of_a_tile_that_is_not_full(cuda, nq, nkv, window, sinks):
         assert not ref.isnan().any()
         for T in (1, 31, 33, 97, 129, 250):
             assert torch.equal(run(T, gt), ref[:T]), T
+
+
+@pytest.mark.parametrize("cta_pairs", [True, False])
+@pytest.mark.parametrize("act,out_t", [(BF, BF), (BF, torch.float32), (torch.float32, torch.float32)])
+def test_contiguous_rows_of_a_tile_that_is_not_full(cuda, cta_pairs, act, out_t):
+    """The same for gqa_prefill, with its two kernels."""
+    g = gen(41)
+    p0, full, nq, nkv = 40, 256, 24, 4
+    rope = ops.rope_table(512)
+    w = torch.ones(HD, device="cuda")
+    x = [normal(g, full, m, HD).to(act) for m in (nq, nkv, nkv, nq)]
+    rows = normal(g, 2, nkv, 512, HD).to(BF)
+
+    def run(T):
+        kc, vc = rows[0].clone(), rows[1].clone()
+        out = torch.full((T + 3, nq, HD), float("nan"), device="cuda", dtype=out_t)
+        ops.gqa_prefill(*(t[:T] for t in x), w, w, rope, kc, vc, out[:T], p0=p0, cta_pairs=cta_pairs)
+        torch.cuda.synchronize()
+        assert ops.device_status() == 0
+        assert out[T:].isnan().all()
+        return out[:T]
+    ref = run(full)
+    assert not ref.isnan().any()
+    for T in (1, 31, 33, 97, 129, 250):
+        assert torch.equal(run(T), ref[:T]), T

@@ -420,6 +420,7 @@ __device__ __forceinline__ void softmax_role(Smem &sm, const Sync &sy, uint32_t 
 #pragma unroll 1
         for (int i = 0; i < HDP / 128; i++) {  // 64 columns per load round
             float o[64];
+            __syncwarp();  // rows past T have skipped the stores; the load wants the whole warp
             tmem_ld64(tO + lane_off + hf * (HDP / 2) + 64 * i, o);
             if (t_row >= T) continue;
 #pragma unroll
