@@ -3,7 +3,7 @@ are in the call, nor on what the other rows of its tile hold."""
 import pytest
 import torch
 
-from test_paged_gpu import BF, HD, Pool, gen, normal
+from test_paged_gpu import BF, HD, Pool, gen, normal, prompt_ref, run_prompt
 from vx27_b200 import ops
 
 pytestmark = pytest.mark.gpu
@@ -58,3 +58,39 @@ def test_contiguous_rows_of_a_tile_that_is_not_full(cuda, cta_pairs, act, out_t)
     assert not ref.isnan().any()
     for T in (1, 31, 33, 97, 129, 250):
         assert torch.equal(run(T), ref[:T]), T
+
+
+def paged_prompt_error(T, s0, at, window=0, gate=True, nq=24, nkv=4):
+    """Largest |error| over its bound of T rows with the same q after s0 slots, where the slots
+    in `at` score 128, 256, ... (all heads) against about 4 at most elsewhere. The bound is
+    prompt_ref's, whose score term grows with the scores' size."""
+    g = gen(42)
+    pool = Pool(g, [s0 + T], nkv, 64)
+    q = normal(g, nkv, HD).to(BF)
+    for i, slot in enumerate(at):
+        page, row = pool.where(0, [slot])
+        pool.k[page, :, row] = (q * (8 * (i + 1)))[None]
+    q = q.repeat_interleave(nq // nkv, 0).expand(T, nq, HD).contiguous()
+    gt = normal(g, T, nq, HD).to(BF) if gate else None
+    got = run_prompt(pool, q, gt, s0, window, 4 if window else 0)
+    ref, tol = prompt_ref(pool, q, gt, s0, window, 4 if window else 0)
+    return float(((got.double() - ref).abs() / tol).max())
+
+
+@pytest.mark.parametrize("T", [1, 64])
+@pytest.mark.parametrize("s0,at,window", [
+    (300, [200], 0),                            # one outlier, in the second tile of an uncut pair
+    (700, [200, 500, 690], 0),                  # each further above the one before
+    (700, [200, 500, 600], 300),                # behind the sinks' tile
+    (20000, [1000, 7000, 13000, 19000], 0)])    # a pair that is cut into parts
+def test_paged_maximum_that_leaves_all_before_it_behind(cuda, T, s0, at, window):
+    """A key tile whose maximum is more than 2^126 times what came before: the sums of the
+    earlier tiles are rescaled to nothing, as their weights underflow."""
+    for gate in (True, False):
+        assert paged_prompt_error(T, s0, at, window, gate) <= 1
+
+
+def test_paged_maximum_odd_heads(cuda):
+    """Pairs of two row tiles (an odd group of heads)."""
+    for T, s0, at in ((1, 300, [200]), (300, 300, [200, 310, 450])):
+        assert paged_prompt_error(T, s0, at, nq=5, nkv=1) <= 1

@@ -321,13 +321,14 @@ __device__ __forceinline__ void softmax_role(Smem &sm, const Sync &sy, const Pro
         if (!last && ok) {
             const float mt = fmaxf(mloc, mpart) * sc2;
             float alpha = 1.0f;
-            const bool grow = mt > m_run + RESCALE_LOG2;
+            const bool grow = mt > m_run + RESCALE_LOG2, seen = m_run != -INFINITY;
             if (grow) {
-                alpha = (m_run == -INFINITY) ? 0.0f : ex2_approx(m_run - mt);
+                alpha = seen ? ex2_approx(m_run - mt) : 0.0f;
                 m_run = mt;
             }
-            // a row that has seen nothing yet has O = 0, and nothing to rescale
-            if (__any_sync(0xffffffffu, grow && alpha > 0.0f)) {
+            // a row that has seen nothing yet has O = 0, and nothing to rescale; alpha of one
+            // that has may underflow to 0, which clears its O
+            if (__any_sync(0xffffffffu, grow && seen)) {
                 ok = sy.wait(&sm.pv_done[b ^ 1], ((g - 1) >> 1) & 1, VX_DEV_TIMEOUT_MMA);
                 ok = __all_sync(0xffffffffu, ok);
                 if (ok) {
