@@ -94,3 +94,34 @@ def test_paged_maximum_odd_heads(cuda):
     """Pairs of two row tiles (an odd group of heads)."""
     for T, s0, at in ((1, 300, [200]), (300, 300, [200, 310, 450])):
         assert paged_prompt_error(T, s0, at, nq=5, nkv=1) <= 1
+
+
+@pytest.mark.parametrize("cta_pairs", [True, False])
+@pytest.mark.parametrize("act", [BF, torch.float32])
+@pytest.mark.parametrize("T", [1, 64])
+def test_contiguous_maximum_that_leaves_all_before_it_behind(cuda, T, act, cta_pairs):
+    """The same for gqa_prefill. With norm weights of 3 and no rotation (cosines 1, sines 0), a
+    key like q scores 9 * 256 / 16 = 144 and the others sqrt(81) = 9 sigma, so below 60 among a
+    few hundred: the outlier's weight is 1 to within e^-80, and a row is its V row times the
+    gate's sigmoid. Its weight, at most 2^8 (the maximum may lag by that), is rounded to bf16
+    and its sum is not: 2^-8; the sigmoid 2^-20."""
+    g = gen(43)
+    p0, at, nq, nkv = 300, 200, 24, 4
+    w = torch.full((HD,), 3.0, device="cuda")
+    rope = torch.cat([torch.ones(512, 32, device="cuda"), torch.zeros(512, 32, device="cuda")], 1)
+    q = normal(g, nkv, HD).to(act)
+    k, v = (normal(g, p0 + T, nkv, HD).to(act) for _ in range(2))
+    k[at] = q
+    q = q.repeat_interleave(nq // nkv, 0)
+    gate = normal(g, p0 + T, nq, HD).to(act)
+    kc, vc = (torch.zeros(nkv, 512, HD, device="cuda", dtype=BF) for _ in range(2))
+    out = torch.empty(p0 + T, nq, HD, device="cuda")
+    for a, b in ((0, p0), (p0, p0 + T)):
+        ops.gqa_prefill(q.expand(b - a, nq, HD).contiguous(), k[a:b], v[a:b], gate[a:b], w, w, rope,
+                        kc, vc, out[a:b], p0=a, cta_pairs=cta_pairs)
+    torch.cuda.synchronize()
+    assert ops.device_status() == 0
+    ref = v[at].to(BF).double().repeat_interleave(nq // nkv, 0) * torch.sigmoid(gate.double())
+    err = (out.double() - ref).abs()[at:]  # of both calls' rows
+    worst = float((err / ((2.0 ** -8 + 2.0 ** -18) * ref.abs()[at:] + 1e-30)).max())
+    assert worst <= 1

@@ -345,9 +345,9 @@ __device__ __forceinline__ void softmax_role(Smem &sm, const Sync &sy, uint32_t 
             m_run = mt;
         }
         // rescale this warp's half of its O rows when one of its rows raised its max (not
-        // on the first tile of a row, where O holds nothing yet), once O += P(j-1) V(j-1)
-        // is done
-        const bool need = grow && alpha > 0.0f;
+        // on the first tile, where O holds nothing yet), once O += P(j-1) V(j-1) is done;
+        // alpha may underflow to 0, which clears O
+        const bool need = grow && j > 0;
         if (__any_sync(0xffffffffu, need)) {
             ok = pf_wait(sy, &sm.pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1, VX_DEV_TIMEOUT_MMA);
             ok = __all_sync(0xffffffffu, ok);
