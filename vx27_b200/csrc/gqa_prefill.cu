@@ -420,31 +420,32 @@ __device__ __forceinline__ void softmax_role(Smem &sm, const Sync &sy, uint32_t 
 #pragma unroll 1
         for (int i = 0; i < HDP / 128; i++) {  // 64 columns per load round
             float o[64];
-            __syncwarp();  // rows past T have skipped the stores; the load wants the whole warp
             tmem_ld64(tO + lane_off + hf * (HDP / 2) + 64 * i, o);
-            if (t_row >= T) continue;
+            if (t_row < T) {
 #pragma unroll
-            for (int k = 0; k < 8; k++) {  // 8 columns per 16-byte gate word group
-                const uint4 gv = graw[8 * i + k];
-                const uint32_t gw4[4] = {gv.x, gv.y, gv.z, gv.w};
-                float a[8];
+                for (int k = 0; k < 8; k++) {  // 8 columns per 16-byte gate word group
+                    const uint4 gv = graw[8 * i + k];
+                    const uint32_t gw4[4] = {gv.x, gv.y, gv.z, gv.w};
+                    float a[8];
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float g0 = bf16_to_f32(gw4[e] & 0xffffu), g1 = bf16_to_f32(gw4[e] >> 16);
-                    a[2 * e] = o[8 * k + 2 * e] * inv * __fdividef(1.0f, 1.0f + __expf(-g0));
-                    a[2 * e + 1] = o[8 * k + 2 * e + 1] * inv * __fdividef(1.0f, 1.0f + __expf(-g1));
-                }
-                const size_t oi = obase + 64 * i + 8 * k;
-                if constexpr (OUT_BF16) {
-                    *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(out) + oi) =
-                        make_uint4(pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]),
-                                   pack_bf16x2(a[4], a[5]), pack_bf16x2(a[6], a[7]));
-                } else {
-                    float4 *op = reinterpret_cast<float4 *>(static_cast<float *>(out) + oi);
-                    op[0] = make_float4(a[0], a[1], a[2], a[3]);
-                    op[1] = make_float4(a[4], a[5], a[6], a[7]);
+                    for (int e = 0; e < 4; e++) {
+                        const float g0 = bf16_to_f32(gw4[e] & 0xffffu), g1 = bf16_to_f32(gw4[e] >> 16);
+                        a[2 * e] = o[8 * k + 2 * e] * inv * __fdividef(1.0f, 1.0f + __expf(-g0));
+                        a[2 * e + 1] = o[8 * k + 2 * e + 1] * inv * __fdividef(1.0f, 1.0f + __expf(-g1));
+                    }
+                    const size_t oi = obase + 64 * i + 8 * k;
+                    if constexpr (OUT_BF16) {
+                        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(out) + oi) =
+                            make_uint4(pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]),
+                                       pack_bf16x2(a[4], a[5]), pack_bf16x2(a[6], a[7]));
+                    } else {
+                        float4 *op = reinterpret_cast<float4 *>(static_cast<float *>(out) + oi);
+                        op[0] = make_float4(a[0], a[1], a[2], a[3]);
+                        op[1] = make_float4(a[4], a[5], a[6], a[7]);
+                    }
                 }
             }
+            __syncwarp();  // rows past T skip the stores; the next load wants the whole warp
         }
     } else if (ok) {
         // fp32 gate: O / l into a row-major fp32 staging tile over the (now idle) slot
