@@ -225,32 +225,32 @@ __device__ __forceinline__ bool write_rows(Smem &sm, const Sync &sy, const Promp
 #pragma unroll 1
     for (int i = 0; i < HD / 64; i++) {
         float o[32];
-        __syncwarp();  // rows past T have skipped the stores; the loads want the whole warp
+        __syncwarp();  // rows past T store nothing; the loads want the whole warp
         tmem_ld16(to + 32 * i, o);
         tmem_ld16(to + 32 * i + 16, o + 16);
         if (!whole) {
             float4 *d = reinterpret_cast<float4 *>(a.rec_o + rec_row * HD + hf * (HD / 2) + 32 * i);
 #pragma unroll
             for (int e = 0; e < 8; e++) d[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-        } else if (t_row < a.T) {
+            continue;
+        }
 #pragma unroll
-            for (int e = 0; e < 4; e++) gate[e] = next[e];
-            if (gated && i < HD / 64 - 1) request(i + 1);
+        for (int e = 0; e < 4; e++) gate[e] = next[e];
+        if (gated && i < HD / 64 - 1) request(i + 1);
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                float x[8];
+        for (int q = 0; q < 4; q++) {
+            float x[8];
 #pragma unroll
-                for (int e = 0; e < 8; e++) x[e] = o[8 * q + e] * inv;
-                if (gated) {
-                    const uint32_t gw[4] = {gate[q].x, gate[q].y, gate[q].z, gate[q].w};
+            for (int e = 0; e < 8; e++) x[e] = o[8 * q + e] * inv;
+            if (gated) {
+                const uint32_t gw[4] = {gate[q].x, gate[q].y, gate[q].z, gate[q].w};
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        x[2 * e] *= __fdividef(1.0f, 1.0f + __expf(-bf16_to_f32(gw[e] & 0xffffu)));
-                        x[2 * e + 1] *= __fdividef(1.0f, 1.0f + __expf(-bf16_to_f32(gw[e] >> 16)));
-                    }
+                for (int e = 0; e < 4; e++) {
+                    x[2 * e] *= __fdividef(1.0f, 1.0f + __expf(-bf16_to_f32(gw[e] & 0xffffu)));
+                    x[2 * e + 1] *= __fdividef(1.0f, 1.0f + __expf(-bf16_to_f32(gw[e] >> 16)));
                 }
-                st8_bf16(a.out + base + 32 * i + 8 * q, x);
             }
+            if (t_row < a.T) st8_bf16(a.out + base + 32 * i + 8 * q, x);
         }
     }
     tc_fence_before();
@@ -321,14 +321,14 @@ __device__ __forceinline__ void softmax_role(Smem &sm, const Sync &sy, const Pro
         if (!last && ok) {
             const float mt = fmaxf(mloc, mpart) * sc2;
             float alpha = 1.0f;
-            const bool grow = mt > m_run + RESCALE_LOG2, seen = m_run != -INFINITY;
+            const bool grow = mt > m_run + RESCALE_LOG2;
             if (grow) {
-                alpha = seen ? ex2_approx(m_run - mt) : 0.0f;
+                alpha = ex2_approx(m_run - mt);
                 m_run = mt;
             }
-            // a row that has seen nothing yet has O = 0, and nothing to rescale; alpha of one
-            // that has may underflow to 0, which clears its O
-            if (__any_sync(0xffffffffu, grow && seen)) {
+            // not on a pair's first tile, where O holds nothing yet; alpha may be 0 (a row that
+            // has seen nothing, or whose weights underflow), which clears O
+            if (__any_sync(0xffffffffu, grow && i > 0)) {
                 ok = sy.wait(&sm.pv_done[b ^ 1], ((g - 1) >> 1) & 1, VX_DEV_TIMEOUT_MMA);
                 ok = __all_sync(0xffffffffu, ok);
                 if (ok) {
