@@ -238,3 +238,45 @@ def test_layer_refuses_a_prompt_without_room():
     for seq, slot, n in ((1, 0, 21), (1, 15, 6), (1, -1, 5), (0, 0, 1), (-1, 0, 1)):
         with pytest.raises(ops.Vx27Error, match="prompt_paged"):
             layer.prompt_paged(torch.zeros(n, 8), c, 0, seq, slot, slot, None)
+
+
+@pytest.mark.parametrize("fails", ["kept", 0, 1])
+def test_an_eviction_that_fails_changes_nothing(monkeypatch, fails):
+    """Memory that runs out before the first layer, or a call refused in a layer: pages, tables,
+    lengths and sums stay as they were, and the eviction succeeds when called again."""
+    from vx27_b200 import paged
+    c = cache(weights=True, n_pages=12)
+    c.extend({0: 60, 2: 33})
+    c.extend({1: 1})
+    c.sums.copy_(torch.rand(c.sums.shape))
+    sums, free = c.sums.clone(), list(c._free)
+    calls = []
+
+    def kv_evict(k, v, table, lens, s, table_out, lens_out, s_out, kept, keep, sinks, recent):
+        if broken and len(calls) == fails:
+            raise ops.Vx27Error("refused")
+        calls.append(table_out.tolist())
+        lens_out.fill_(keep)
+        s_out.fill_(7)
+        kept.fill_(len(calls))
+
+    def empty(*shape, **kw):
+        if broken and fails == "kept":
+            raise torch.OutOfMemoryError("no memory")
+        return make(*shape, **kw)
+    make, broken = torch.empty, True
+    monkeypatch.setattr(paged.ops, "kv_evict", kv_evict)
+    monkeypatch.setattr(paged.torch, "empty", empty)
+    with pytest.raises((ops.Vx27Error, torch.OutOfMemoryError)):
+        c.evict(20, sinks=2, recent=4)
+    assert c._free == free and torch.equal(c.sums, sums) and c._lens == [60, 1, 33]
+    held(c)
+    broken = False
+    calls.clear()
+    cut, kept = c.evict(20, sinks=2, recent=4)
+    assert cut == [0, 2] and kept[:, 0, 0, 0].tolist() == [1, 2]
+    assert c._lens == [20, 1, 20] and len(held(c)) == 5
+    assert all(t == [c._pages[0][:2], c._pages[2][:2]] for t in calls) and len(calls) == 2
+    for s in (0, 2):
+        assert (c.sums[:, s, :, :32] == 7).all() and (c.sums[:, s, :, 32:] == 0).all()
+    assert torch.equal(c.sums[:, 1], sums[:, 1])

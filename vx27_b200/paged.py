@@ -156,20 +156,23 @@ class PagedKV:
         if n * len(cut) > len(self._free):
             raise Vx27Error(f"PagedKV: evict needs {n * len(cut)} free pages, {len(self._free)} are")
         layers, nkv, dev = len(self.k), self.k.shape[2], self.k.device
-        new = [[self._free.pop() for _ in range(n)] for _ in cut]
+        # the pages leave the free list, and the sums change, once every layer's call is made
+        take = n * len(cut)
+        free = self._free[:-take - 1:-1]
+        new = [free[i * n:(i + 1) * n] for i in range(len(cut))]
         rows = torch.tensor(cut, device=dev)
         dst = torch.tensor(new, dtype=torch.int32, device=dev)
         table, lens = self.table[rows], self.lens[rows]
         lens_out = torch.empty_like(lens)
         kept = torch.empty(layers, len(cut), nkv, keep, dtype=torch.int32, device=dev)
-        out = torch.empty(len(cut), nkv, n * self.page_size, device=dev)
+        out = torch.empty(layers, len(cut), nkv, n * self.page_size, device=dev)
         for i in range(layers):
-            sums = self.sums[i, rows]
-            ops.kv_evict(self.k[i], self.v[i], table, lens, sums, dst, lens_out, out, kept[i], keep,
-                         sinks=sinks, recent=recent)
-            self.sums[i, rows] = 0
-            self.sums[i, rows, :, :n * self.page_size] = out
-        for s, pages in zip(cut, new):
+            ops.kv_evict(self.k[i], self.v[i], table, lens, self.sums[i, rows], dst, lens_out, out[i],
+                         kept[i], keep, sinks=sinks, recent=recent)
+        del self._free[-take:]
+        for j, (s, pages) in enumerate(zip(cut, new)):
+            self.sums[:, s] = 0
+            self.sums[:, s, :, :n * self.page_size] = out[:, j]
             self._free += [p for p in self._pages[s] if p >= 0]
             self._pages[s] = pages + [-1] * (self.max_pages - n)
             self._lens[s] = keep
