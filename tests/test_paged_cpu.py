@@ -280,3 +280,36 @@ def test_an_eviction_that_fails_changes_nothing(monkeypatch, fails):
     for s in (0, 2):
         assert (c.sums[:, s, :, :32] == 7).all() and (c.sums[:, s, :, 32:] == 0).all()
     assert torch.equal(c.sums[:, 1], sums[:, 1])
+
+
+def test_a_prompt_of_one_token_is_no_lane():
+    """extend(prompts=...): the device's step entry stays 0 for a prompt's single token, and
+    prompt_paged refuses a token that is a lane of step_paged, which would store it a second time."""
+    from vx27_b200.layer import GQALayer
+    layer, c = object.__new__(GQALayer), cache()
+    c.extend({0: 5, 1: 20})
+    c.extend({0: 1, 1: 1, 2: 1}, prompts=[1, 2])
+    assert c.step.tolist() == [6, 0, 0]
+    held(c)
+    with pytest.raises(ops.Vx27Error, match="lane of step_paged"):
+        layer.prompt_paged(torch.zeros(1, 8), c, 0, 0, 5, 5, None)
+    with pytest.raises(ops.Vx27Error, match="lane of step_paged"):
+        layer.prompt_paged(torch.zeros(3, 8), c, 0, 0, 3, 3, None)
+    before = c._lens[:]
+    for prompts in ([1], [3], [-1], [0, 2]):
+        with pytest.raises(ops.Vx27Error, match="prompts"):
+            c.extend({0: 1, 2: 3} if prompts != [0, 2] else {0: 1}, prompts=prompts)
+    assert c._lens == before and c.step.tolist() == [6, 0, 0]
+
+    class Reached(Exception):
+        pass
+
+    def project(*a):
+        raise Reached
+    layer._project = project
+    for seq, slot, n in ((1, 20, 1), (1, 0, 21), (2, 0, 1), (0, 0, 5)):  # prompts, earlier slots
+        with pytest.raises(Reached):
+            layer.prompt_paged(torch.zeros(n, 8), c, 0, seq, slot, slot, None)
+    c.extend({2: 4})  # a later call's lanes alone count
+    with pytest.raises(Reached):
+        layer.prompt_paged(torch.zeros(1, 8), c, 0, 0, 5, 5, None)

@@ -126,10 +126,10 @@ class GQALayer:
 
     def step_paged(self, x: torch.Tensor, cache, layer: int,
                    workspace: torch.Tensor) -> torch.Tensor:
-        """One token of each sequence of a paged.PagedKV that its last extend() gave one to: x
-        [B, H] fp32. The other lanes are idle: they store nothing and their rows come from a
-        zero attention output. With weights=True the layer's weight sums grow. Returns [B, H]
-        fp32."""
+        """One token of each sequence of a paged.PagedKV that its last extend() gave one to, but
+        for its prompts: x [B, H] fp32. The other lanes are idle: they store nothing and their
+        rows come from a zero attention output. With weights=True the layer's weight sums grow.
+        Returns [B, H] fp32."""
         q_in, gate, k, v = self._project(x, None)
         q = torch.empty_like(q_in)
         idle = cache.step == 0
@@ -145,11 +145,15 @@ class GQALayer:
     def prompt_paged(self, x: torch.Tensor, cache, layer: int, seq: int, slot: int, pos: int,
                      workspace: torch.Tensor) -> torch.Tensor:
         """T prompt tokens of one sequence of a paged.PagedKV, whose extend() has made room for
-        them at (slot, pos): x [T, H] fp32. The attention runs in bf16. Returns [T, H] fp32."""
+        them at (slot, pos): x [T, H] fp32. A prompt of one token has to be one of extend's
+        prompts, else step_paged takes it. The attention runs in bf16. Returns [T, H] fp32."""
         T = x.shape[0]
         if seq < 0 or slot < 0 or slot + T > cache.length(seq):
             raise ops.Vx27Error(f"prompt_paged: {T} tokens from slot {slot}, sequence {seq} holds "
                                 f"{cache.length(seq)}")
+        if cache.is_lane(seq) and slot + T == cache.length(seq):
+            raise ops.Vx27Error(f"prompt_paged: the last token of sequence {seq} is a lane of "
+                                "step_paged; name the sequence in extend's prompts")
         q_in, gate, k, v = self._project(x, None)
         at = torch.arange(T, dtype=torch.int32, device=x.device)
         q = torch.empty(q_in.shape, dtype=torch.bfloat16, device=x.device)

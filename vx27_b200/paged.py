@@ -8,12 +8,16 @@ where, so nothing is read back. Per sequence the device holds (int32)
 
     lens   slots held
     pos    positions taken; equal to lens until an eviction cuts the slots back
-    step   lens, if the last extend() gave the sequence one token, else 0 (an idle lane)
+    step   lens, if the last extend() gave the sequence one token that is no prompt's, else 0 (an
+           idle lane of step_paged)
 
 ``layer.GQALayer.step_paged`` and ``prompt_paged`` run a layer over it. A round of a server:
 
-    at = cache.extend({0: 1, 1: 1, 5: 300})       # two running sequences, a new prompt
+    at = cache.extend({0: 1, 1: 1, 5: n}, prompts=[5])   # two running sequences, a new prompt
     for each layer i: step_paged(x, cache, i, ws), prompt_paged(xp, cache, i, 5, *at[5], ws)
+
+A token enters the cache once: by step_paged, or by prompt_paged for the sequences that extend()
+was told to be prompts, which matters where a prompt, or its last piece, is one token long.
 
 The tensors keep their addresses, so a captured step_paged may be replayed after each
 extend(); extend, release and evict copy from the host and stay outside the capture. All
@@ -52,6 +56,7 @@ class PagedKV:
         self._free = list(range(n_pages - 1, -1, -1))
         self._pages = [[-1] * max_pages for _ in range(batch)]
         self._lens, self._pos = [0] * batch, [0] * batch
+        self._lanes = set()  # sequences whose token the next step_paged takes
 
     # ------------------------------------------------------------------ bookkeeping (host)
     @property
@@ -63,6 +68,10 @@ class PagedKV:
 
     def position(self, seq: int) -> int:
         return self._pos[seq]
+
+    def is_lane(self, seq: int) -> bool:
+        """Does the sequence's last token go through step_paged?"""
+        return seq in self._lanes
 
     def _check(self, seqs) -> None:
         seqs = list(seqs)
@@ -84,8 +93,9 @@ class PagedKV:
         for s in seqs:
             self.table[s].copy_(torch.tensor(self._pages[s], dtype=torch.int32))
 
-    def _upload_state(self, step: dict[int, int]) -> None:
-        one = [n if step.get(s) == 1 else 0 for s, n in enumerate(self._lens)]
+    def _upload_state(self, lanes=()) -> None:
+        self._lanes = set(lanes)
+        one = [n if s in self._lanes else 0 for s, n in enumerate(self._lens)]
         self._state.copy_(torch.tensor([self._lens, self._pos, one], dtype=torch.int32))
 
     def _out_of_sight(self, seq: int) -> list[int]:
@@ -96,12 +106,16 @@ class PagedKV:
         first = -(-self.sinks // ps)
         return [e for e in range(first, max(lo, 0) // ps) if self._pages[seq][e] >= 0]
 
-    def extend(self, tokens: dict[int, int]) -> dict[int, tuple[int, int]]:
+    def extend(self, tokens: dict[int, int], prompts=()) -> dict[int, tuple[int, int]]:
         """Makes room for tokens[seq] more tokens of each sequence and counts them as held:
         (first slot, first position) by sequence. Pages that earlier calls moved out of sight of
         a window are freed first. On the device the state is that after these tokens; a
-        sequence that gets one token takes part in the next step_paged, the others do not."""
+        sequence that gets one token takes part in the next step_paged, unless it is one of
+        prompts, whose tokens go through prompt_paged. The others do not."""
         self._check(tokens)
+        prompts = set(prompts)
+        if not prompts <= tokens.keys():
+            raise Vx27Error(f"PagedKV: prompts {sorted(prompts)} among tokens of {sorted(tokens)}")
         need = {s: self._need(s, n) for s, n in tokens.items()}
         changed = set()
         for s in tokens:
@@ -122,7 +136,7 @@ class PagedKV:
             self._lens[s] += n
             self._pos[s] += n
         self._upload(changed)
-        self._upload_state(tokens)
+        self._upload_state(s for s, n in tokens.items() if n == 1 and s not in prompts)
         return at
 
     def release(self, seq: int) -> None:
@@ -132,7 +146,7 @@ class PagedKV:
         self._pages[seq] = [-1] * self.max_pages
         self._lens[seq] = self._pos[seq] = 0
         self._upload([seq])
-        self._upload_state({})
+        self._upload_state()
         if self.sums is not None:
             self.sums[:, seq] = 0
 
@@ -177,7 +191,7 @@ class PagedKV:
             self._pages[s] = pages + [-1] * (self.max_pages - n)
             self._lens[s] = keep
         self._upload(cut)
-        self._upload_state({})
+        self._upload_state()
         return cut, kept
 
     def workspace(self, nq: int) -> torch.Tensor:
