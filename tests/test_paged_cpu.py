@@ -313,3 +313,19 @@ def test_a_prompt_of_one_token_is_no_lane():
     c.extend({2: 4})  # a later call's lanes alone count
     with pytest.raises(Reached):
         layer.prompt_paged(torch.zeros(1, 8), c, 0, 0, 5, 5, None)
+
+
+def test_lanes_outlive_what_happens_to_other_sequences(monkeypatch):
+    """release and evict between extend and step_paged idle the sequences that they change, and
+    leave the others' lanes."""
+    from vx27_b200 import paged
+    c = cache(weights=True, batch=4, n_pages=20)
+    c.extend({0: 3, 1: 40, 2: 50, 3: 3})
+    c.extend({0: 1, 1: 1, 2: 1, 3: 1}, prompts=[3])
+    assert c.step.tolist() == [4, 41, 51, 0]
+    c.release(1)
+    assert c.step.tolist() == [4, 0, 51, 0] and c.is_lane(0) and not c.is_lane(1)
+    monkeypatch.setattr(paged.ops, "kv_evict", lambda *a, **kw: None)
+    assert c.evict(20)[0] == [2]
+    assert c.step.tolist() == [4, 0, 0, 0] and c.is_lane(0) and not c.is_lane(2)
+    held(c)

@@ -93,7 +93,7 @@ class PagedKV:
         for s in seqs:
             self.table[s].copy_(torch.tensor(self._pages[s], dtype=torch.int32))
 
-    def _upload_state(self, lanes=()) -> None:
+    def _upload_state(self, lanes) -> None:
         self._lanes = set(lanes)
         one = [n if s in self._lanes else 0 for s, n in enumerate(self._lens)]
         self._state.copy_(torch.tensor([self._lens, self._pos, one], dtype=torch.int32))
@@ -140,13 +140,13 @@ class PagedKV:
         return at
 
     def release(self, seq: int) -> None:
-        """The sequence is done: its pages are free, its lane is idle."""
+        """The sequence is done: its pages are free, its lane is idle (the others stay)."""
         self._check([seq])
         self._free += [p for p in self._pages[seq] if p >= 0]
         self._pages[seq] = [-1] * self.max_pages
         self._lens[seq] = self._pos[seq] = 0
         self._upload([seq])
-        self._upload_state()
+        self._upload_state(self._lanes - {seq})
         if self.sums is not None:
             self.sums[:, seq] = 0
 
@@ -155,8 +155,8 @@ class PagedKV:
         """Cuts the sequences that hold more than keep slots (all, or those of seqs) back to keep
         of them in every layer and head: the first sinks, the last recent, and those with the
         largest summed weights (vx27_kv_evict). They need ceil(keep / page_size) free pages each
-        meanwhile; their old pages are free afterwards. Returns the sequences cut and their kept
-        slots [layers][n][nkv][keep]."""
+        meanwhile; their old pages are free and their lanes idle afterwards. Returns the sequences
+        cut and their kept slots [layers][n][nkv][keep]."""
         if self.sums is None:
             raise Vx27Error("PagedKV: evict needs weights=True")
         seqs = range(len(self._lens)) if seqs is None else list(seqs)
@@ -191,7 +191,7 @@ class PagedKV:
             self._pages[s] = pages + [-1] * (self.max_pages - n)
             self._lens[s] = keep
         self._upload(cut)
-        self._upload_state()
+        self._upload_state(self._lanes - set(cut))
         return cut, kept
 
     def workspace(self, nq: int) -> torch.Tensor:
