@@ -576,6 +576,7 @@ dn_scan_tc(Wsp ws, float *__restrict__ S, int n_chunks, uint32_t *status) {
         if (lane == 0) load_stage(0);
         for (int c = 0; c < n_chunks; c++) {
             const size_t blk = (size_t)vh * n_chunks + c;
+            __syncwarp();  // the barriers want whole warps
             named_bar_sync(SCAN_BAR_A, 160);
             if (lane == 0) {
                 // the state at this chunk's start -> S0^T images for the output kernel
@@ -591,6 +592,7 @@ dn_scan_tc(Wsp ws, float *__restrict__ S, int n_chunks, uint32_t *status) {
                 if (c + 1 < n_chunks && !*abort_) load_stage(c + 1);
                 bulk_wait_read0();  // S0 images out before the state operand is rewritten
             }
+            __syncwarp();
             named_bar_sync(SCAN_BAR_B, 160);
             if (lane == 0) {
                 bulk_s2g(ws.UH + blk * SZ_U + cb * CB * 128, UB, CB * 128);
@@ -650,6 +652,7 @@ dn_scan_tc(Wsp ws, float *__restrict__ S, int n_chunks, uint32_t *status) {
             }
         }
         if (!*abort_ && !mbar_wait(&bars[2], c & 1, status, VX_DEV_TIMEOUT_MMA)) *abort_ = 1;
+        __syncwarp();  // lane 0 comes from the issue, and the loads want the whole warp
         tc_fence_after();
         // U = Wv - (quadrant sums): own half kept, the other half handed to thread tid ^ 64
         const float *wv_s = reinterpret_cast<const float *>(stage + Lay::ST_WV);
@@ -715,6 +718,7 @@ dn_scan_tc(Wsp ws, float *__restrict__ S, int n_chunks, uint32_t *status) {
             mma_commit(&bars[3]);
         }
         if (!*abort_ && !mbar_wait(&bars[3], c & 1, status, VX_DEV_TIMEOUT_MMA)) *abort_ = 1;
+        __syncwarp();
         tc_fence_after();
         constexpr int SJ = CB < 16 ? CB : 16;
 #pragma unroll
