@@ -64,7 +64,8 @@ int vx27_gqa_paged_append(const void *q_in, const void *k_in, const void *v_in,
  *   with VX27_F_OUT_BF16)
  *   weight_sum fp32 [B][nkv][max_pages * page_size] or NULL: to the entry of each slot attended
  *   to, the softmax weights that the heads of its group gave it are added (vx27_kv_evict)
- *   workspace: vx27_gqa_paged_workspace_size(...) bytes, 16-byte aligned
+ *   workspace: vx27_gqa_paged_workspace_size(...) bytes, 16-byte aligned; with weight sums it
+ *   holds B * nq * max_slots floats (with a window only as many slots as that and the sinks span)
  * The slots that the batch attends to are counted in tiles of 128 and cut into n_parts equal
  * runs (0: one per SM; at most 1024), which are joined where a cut goes through a sequence. So the
  * lengths of the other sequences move the cuts, and with them the last bits of a result; the

@@ -18,8 +18,9 @@ constexpr int HD = PG_HD;
 // partners rope_dim / 2 + 4 l .., the others 8 l .., so a rotation needs no other lane; lanes
 // without one rotate by (1, 0). The square sum is a tree of fp32 sums.
 // Bound by the activations' bytes when there are many tokens: 4096 tokens of 24 + 4 heads take
-// 32 us, 4.2 TB/s (one head per warp at a time, everything looked up per head: 53 us); one
-// token takes 3.1 us, the chain slot -> page -> store.
+// 31 us, 4.3 TB/s (one head per warp at a time, everything looked up per head: 53 us; a plain
+// copy of the bytes: 24 us). Their 2048 blocks run in 2.3 rounds of 6 per SM, each with the chain
+// of lookups in front. One token takes 3.1 us, the chain slot -> page -> store.
 constexpr int APPEND_THREADS = 128;
 struct AppendArgs {
     const void *q_in, *k_in, *v_in;

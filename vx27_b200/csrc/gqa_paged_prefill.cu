@@ -26,8 +26,15 @@
 // What bounds it: the tensor cores and the softmax warps that feed them (4 T_keys 128 256 FLOP
 // per row tile); K and V come from L2, which the heads of a KV head share. 2048 rows after 14001
 // slots take 570 us at 1965 MHz (1330 TFLOP/s, 0.81 of the cuBLAS rate; 1.8 us a key tile of a
-// pair) and 680 under the power cap; 300 rows after 130, one round, 22 us, of which the last
-// pair's rows are 5: two SFU operations per gate and 32 rows an access.
+// pair) and 650-670 under the power cap; 300 rows after 130, one round, 20 us, of which the last
+// pair's rows are 5: two SFU operations per gate and 32 rows an access. A tile holds rows of one
+// head, so few rows leave most of it empty: one row after 8000 slots takes 46 us, 8 rows 48,
+// against 5 for the bytes.
+//
+// p is rounded to bf16, half a step of 2^-8 relative, and l sums it unrounded: results are off by
+// 2.1e-3 to 2.4e-3 of their size, of which their own rounding to bf16 makes 1.7e-3. A second
+// term of p would take as many O MMAs again (half as many tensor operations more in all), and
+// tensor memory is full.
 //
 // Warps of a CTA: 0 copies K (and Q), 11 copies V, 1 S MMAs, 10 O MMAs, 2-9 softmax (two
 // threads a row, one per half of the keys and of the output columns). Rank 0 issues the

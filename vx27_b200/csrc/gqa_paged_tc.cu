@@ -469,7 +469,7 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
             int g = 0, kq = 0, sl = 0;
             uint32_t phase = 0;
             Walk w = start;
-                for (; !w.done() && ok; w.next(), kq++) {
+            for (; !w.done() && ok; w.next(), kq++) {
                 const uint64_t dq = sdesc_add(dq0, (kq % QB) * (uint32_t)sizeof(sm.q[0]));
                 ok = bar_wait(&sm.q_full[kq % QB], (kq / QB) & 1, &sm.abort, status, VX_DEV_TIMEOUT_MMA);
                 for (int i = 0; i < w.cnt && ok; i++, g++) {
@@ -510,7 +510,7 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
             int g = 0, sl = 0;
             uint32_t phase = 0;
             Walk w = start;
-                for (; !w.done() && ok; w.next()) {
+            for (; !w.done() && ok; w.next()) {
                 for (int i = 0; i < w.cnt && ok; i++, g++) {
                     const int bb = g & 1;
                     const uint32_t seen = w.t.seen_groups(w.t.first_slot(w.v0 + i));
@@ -809,12 +809,15 @@ paged_decode_tc(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
 // 2^(s_h - m_h) / l_h.
 // Nothing but round trips and instructions bound it. The first two records of an item are those
 // of runs c - 1 and c, so they are requested along with the plan. Items of more records take 38
-// more of them per round trip (FEW: at most an eighth as many items as runs) or 4, in
-// fewer registers: one sequence of 8192 slots (37 runs an item) takes 20.8 us in all with FEW and
-// 24.2 without, 4 of them 34.5 and 34.6, 8 of 2112 25.0 and 24.5, 16 of them 37.1 and 36.3.
+// more of them in the first round trip (FEW: at most an eighth as many items as runs), or 4, in
+// fewer registers; what is left after that comes four at a time. Replayed from a graph, one
+// sequence of 8192 slots (37 runs an item) takes 17.3 us in all with FEW and 19.2 without, 4 of
+// them 34.3 and 34.0, 8 of 2112 21.4 and 20.3, 16 of them 37.1 and 35.3. The lengths are on the
+// device, so the rule counts lanes: one such sequence among 64 lanes takes 20.7, with FEW 18.0.
 // WEIGHTS is an instance of its own, whose registers the others need not have; sums are read and
 // written four at a time, requested with the scores (32 ragged sequences 62.5 us in all, 65.7
-// with scalar sums added at the end, 56 without sums).
+// with scalar sums added at the end, 56 without sums). Their blocks, and the scores, are as many
+// as the tables' slots need: the same call with tables of 65536 slots takes 69 us, of 262144 94.
 template <bool FEW, bool WEIGHTS>
 __global__ void __launch_bounds__(256, FEW ? 3 : WEIGHTS ? 4 : 5)
 paged_join_k(const __grid_constant__ DecodeArgs a, int P, int G, int slot_blocks) {

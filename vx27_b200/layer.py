@@ -134,8 +134,8 @@ class GQALayer:
         q = torch.empty_like(q_in)
         idle = cache.step == 0
         ops.gqa_paged_append(q_in, k, v, self.q_norm_w, self.k_norm_w, self.rope,
-                             (cache.pos - 1).masked_fill_(idle, 0), cache.step - 1, cache.table, cache.k[layer], cache.v[layer], q,
-                             eps=self.eps, norm_one_plus=True)
+                             (cache.pos - 1).masked_fill_(idle, 0), cache.step - 1, cache.table,
+                             cache.k[layer], cache.v[layer], q, eps=self.eps, norm_one_plus=True)
         att = torch.empty_like(q)
         ops.gqa_paged_decode(q, gate, cache.k[layer], cache.v[layer], cache.table, cache.step, att,
                              workspace, window=cache.window, sinks=cache.sinks,
