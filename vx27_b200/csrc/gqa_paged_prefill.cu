@@ -411,7 +411,7 @@ paged_prompt_k(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
     const uint32_t rank = cluster_rank();
     const int nkv = a.pool.nkv, group = a.nq / nkv, c = (int)(blockIdx.x >> 1);
 
-    if (tid == 0) {
+    if (tid == 32) {  // not of warp 0, which allocates as a whole
         mbar_init(&sm.qfull, 1);
         mbar_init(&sm.q_empty, 1);
         mbar_init(&sm.o_empty, 16);

@@ -747,6 +747,7 @@ prefill_attn_pair(const __grid_constant__ CUtensorMap tmq, const __grid_constant
         fence_barrier_init();
     }
     if (warp == 0) {
+        __syncwarp();
         tmem_alloc_pair(&sm.tmem_base, 512);
         tmem_relinquish_pair();
         if (lane == 0) { tma_prefetch_desc(&tmq); tma_prefetch_desc(&tmk); tma_prefetch_desc(&tmv); }

@@ -10,8 +10,10 @@
 namespace vx27 {
 
 // ---- TMEM --------------------------------------------------------------------
-// Allocation is warp-wide; the allocated base column lands in *slot (shared memory).
+// Allocation is warp-wide (a warp whose lane 0 has set up barriers meets first); the allocated
+// base column lands in *slot (shared memory).
 __device__ __forceinline__ void tmem_alloc(uint32_t *slot, uint32_t ncols) {
+    __syncwarp();
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                  ::"r"(smem_u32(slot)), "r"(ncols) : "memory");
 }
@@ -214,6 +216,7 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;"
                  ::: "memory");
 }
+// The warp comes whole: cluster-wide setup is left to another one, or it meets first.
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t *slot, uint32_t ncols) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
                  ::"r"(smem_u32(slot)), "r"(ncols) : "memory");
